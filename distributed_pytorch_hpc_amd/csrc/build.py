@@ -24,6 +24,9 @@ BUILD_DIR = os.path.join(PKG, "..", "build", "native")
 OUT = os.path.join(PKG, "_C.so")
 ARCH = os.environ.get("DPH_OFFLOAD_ARCH", "gfx950")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
+# No packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on MI355X now and
+# then, and -O3 forms them from ordinary float code.  The host pass warns that it does not know the feature: harmless.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # attention.hip (the forward): no NaN semantics needed (masks are -inf, never NaN), and IEEE mode off so fmaxf on MFMA
 # results is a bare v_max / v_max3 instead of a canonicalising v_max per operand first (the row max of every score
 # tile): forward 814 -> 836 TFLOP/s.  attention_bwd.hip has no row max and is built WITHOUT them: under these flags
@@ -53,7 +56,7 @@ def write_ninja(build_dir: str, verbose_asm: bool = False) -> str:
     hipcc = os.path.join(ROCM, "bin", "hipcc")
     hip_flags = [
         f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-munsafe-fp-atomics",
-        f"-I{HERE}", "-Wno-unused-result",
+        f"-I{HERE}", "-Wno-unused-result", *NO_PACKED_FP32,
     ]
     if verbose_asm:
         hip_flags.append("-Rpass-analysis=kernel-resource-usage")
