@@ -373,6 +373,53 @@ void gemv(const GemvArgs& a, int xmode, hipStream_t stream);
 void skinny_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, int M, int N, int K,
                  hipStream_t stream);
 
+// Block-scaled 8-bit KV cache (csrc/kv8.hip).  A cache holding n tokens of a sequence in blocks of T tokens keeps the
+// blocks j < n / T as 8-bit codes with one fp32 scale per (block, KV head), value = code * scale, and the n % T rows of
+// the open block as bf16 in the tail (row t % T).  K and V parts have equal strides (elements).
+struct KV8 {
+  void* kc; void* vc; int64_t c_sb, c_ss, c_sh;      // codes [B, Smax, Hkv, D]
+  float* ks; float* vs; int64_t s_sb, s_sn, s_sh;    // scales [B, Smax / T, Hkv]
+  void* kt; void* vt; int64_t t_sb, t_ss, t_sh;      // open block, bf16 [B, T, Hkv, D]
+  int B, Smax, Hkv, D, T;
+  int e4m3;                                          // codes are OCP e4m3, else int8
+};
+struct KV8AppendParams {
+  KV8 c;
+  void* qkv; int64_t qkv_sb, qkv_ss;                 // [B, S, (Hq + 2 Hkv) * D] bf16; q and k rotated in place
+  const int* pos; const float* cos; const float* sin;
+  int S, Hq;
+};
+void kv8_append(const KV8AppendParams& p, hipStream_t stream);
+struct KV8DecodeParams {
+  KV8 c;
+  const void* q; int64_t q_sb;                       // q[b, hq * D + d] bf16
+  const int* pos;                                    // keys 0 .. pos[b] are visible
+  void* out;                                         // bf16 [B, Hq * D]
+  int Hq;
+  float scale;
+};
+void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t stream);
+// rows pos[b] - count .. pos[b] - 1 of every sequence as bf16 [B, count, Hkv, D] (rows before the first token: zero)
+struct KV8ReadParams {
+  KV8 c;
+  const int* pos;
+  void* ko; void* vo; int64_t o_sb, o_ss, o_sh;
+  int count;
+};
+void kv8_read(const KV8ReadParams& p, hipStream_t stream);
+
+// Penalties, biases and masks on a row of logits (csrc/logits.hip); every pointer but x and y may be null.
+struct LogitParams {
+  const void* x; int64_t ldx; void* y;               // [N, V], y contiguous
+  const int64_t* tokens; int64_t ldt; int L;         // history [N, L]
+  const int* lengths; const int* prompt;             // valid ids of a row, and how many of them are the prompt's
+  const float* rep; const float* pres; const float* freq;
+  const float* bias; int64_t ldb;                    // fp32 [N, V] (ldb 0: one row for all)
+  const int* mask; int64_t ldm;                      // bit v % 32 of word v / 32: token v allowed (ldm 0: one row)
+  int N, V;
+};
+void process_logits(const LogitParams& p, int dtype, hipStream_t stream);
+
 // Single-node all-reduce over IPC-mapped peer buffers (csrc/custom_allreduce.hip).  ctx is an opaque handle.
 int64_t car_create(int rank, int world, int64_t max_bytes, double timeout_s);
 void car_ipc_handle(int64_t ctx, void* out64);

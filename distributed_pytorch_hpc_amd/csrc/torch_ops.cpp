@@ -3,6 +3,7 @@
 // ops/*.py.  Every op validates its operands on the host (shape, dtype, contiguity, alignment) before a
 // launch, so a kernel never sees a layout it was not written for.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -502,6 +503,186 @@ Tensor decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, c
   p.kv_fp8 = fp8; p.kv_scale = (float)kv_scale;
   dph::decode_attention(p, cur_stream());
   return out;
+}
+
+// ------------------------------------------------------------------------------- block-scaled 8-bit KV cache, logits
+bool strides_ok(const Tensor& t, int64_t mult) {   // unit stride along the last dim, the others (of real dims) x mult
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) <= 1) continue;
+    if (i == t.dim() - 1 ? t.stride(i) != 1 : t.stride(i) % mult != 0) return false;
+  }
+  return true;
+}
+
+dph::KV8 check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& kt,
+                   const Tensor& vt) {
+  TORCH_CHECK(kc.is_cuda() && kc.dim() == 4 && kt.dim() == 4 && ks.dim() == 3, "kv8: k / v [B, Smax, Hkv, D], scales "
+              "[B, Smax / T, Hkv], tails [B, T, Hkv, D] on the GPU");
+  for (const Tensor* t : {&vc, &ks, &vs, &kt, &vt})
+    TORCH_CHECK(t->device() == kc.device(), "kv8: every part of the cache must be on one device");
+  const bool e4m3 = kc.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK((e4m3 || kc.scalar_type() == at::kChar) && vc.scalar_type() == kc.scalar_type(),
+              "kv8: k and v must both be int8 or float8_e4m3fn");
+  TORCH_CHECK(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat, "kv8: scales must be fp32");
+  TORCH_CHECK(kt.scalar_type() == at::kBFloat16 && vt.scalar_type() == at::kBFloat16, "kv8: tails must be bf16");
+  TORCH_CHECK(kc.sizes() == vc.sizes() && ks.sizes() == vs.sizes() && kt.sizes() == vt.sizes() &&
+                  kc.strides() == vc.strides() && ks.strides() == vs.strides() && kt.strides() == vt.strides(),
+              "kv8: k and v parts must have equal sizes and strides");
+  const int64_t B = kc.size(0), Smax = kc.size(1), H = kc.size(2), D = kc.size(3), T = kt.size(1);
+  TORCH_CHECK(D == 32 || D == 64 || D == 128, "kv8: head_dim must be 32, 64 or 128");
+  TORCH_CHECK(T == 16 || T == 32 || T == 64 || T == 128, "kv8: the block must be 16, 32, 64 or 128 tokens");
+  TORCH_CHECK(kt.size(0) == B && kt.size(2) == H && kt.size(3) == D && ks.size(0) == B && ks.size(1) == Smax / T &&
+                  ks.size(2) == H && Smax >= 1 && Smax < (int64_t(1) << 31) - 256 && H >= 1,
+              "kv8: scales [B, Smax / T, Hkv] and tails [B, T, Hkv, D] must match k / v [B, Smax, Hkv, D]");
+  TORCH_CHECK(strides_ok(kc, 16) && strides_ok(kt, 8),
+              "kv8: head dim contiguous, the other strides multiples of 16 bytes");
+  check_align16(kc, "k"); check_align16(vc, "v"); check_align16(kt, "k_tail"); check_align16(vt, "v_tail");
+  dph::KV8 c{};
+  c.kc = kc.data_ptr(); c.vc = vc.data_ptr(); c.c_sb = kc.stride(0); c.c_ss = kc.stride(1); c.c_sh = kc.stride(2);
+  c.ks = ks.data_ptr<float>(); c.vs = vs.data_ptr<float>();
+  c.s_sb = ks.stride(0); c.s_sn = ks.stride(1); c.s_sh = ks.stride(2);
+  c.kt = kt.data_ptr(); c.vt = vt.data_ptr(); c.t_sb = kt.stride(0); c.t_ss = kt.stride(1); c.t_sh = kt.stride(2);
+  c.B = (int)B; c.Smax = (int)Smax; c.Hkv = (int)H; c.D = (int)D; c.T = (int)T; c.e4m3 = e4m3 ? 1 : 0;
+  return c;
+}
+
+// qkv [B, S, (Hq + 2 Hkv) * D] bf16 of the cache's device
+void check_kv8_qkv(const Tensor& qkv, const dph::KV8& c, const Tensor& kc, int64_t n_heads, int64_t n_kv_heads) {
+  TORCH_CHECK(qkv.device() == kc.device() && qkv.dim() == 3 && qkv.scalar_type() == at::kBFloat16 &&
+                  n_kv_heads == c.Hkv && n_heads >= 1 && n_heads % n_kv_heads == 0 && qkv.size(0) == c.B &&
+                  qkv.size(2) == (n_heads + 2 * n_kv_heads) * c.D,
+              "kv8: qkv must be bf16 [B, S, (Hq + 2 Hkv) * D] on the cache's device, Hq a multiple of Hkv");
+  TORCH_CHECK(strides_ok(qkv, 8), "kv8: qkv needs a contiguous last dim and strides that are multiples of 8");
+  check_align16(qkv, "qkv");
+}
+
+void no_overlap(std::initializer_list<const Tensor*> ts) {   // written operands: none twice in memory, no two the same
+  for (auto a = ts.begin(); a != ts.end(); ++a) {
+    at::assert_no_internal_overlap(**a);
+    for (auto b = ts.begin(); b != a; ++b) at::assert_no_overlap(**a, **b);
+  }
+}
+
+void kv8_append_(Tensor& qkv, Tensor& kc, Tensor& vc, Tensor& ks, Tensor& vs, Tensor& kt, Tensor& vt, const Tensor& pos,
+                 const Tensor& cos, const Tensor& sin, int64_t n_heads, int64_t n_kv_heads) {
+  dph::KV8AppendParams p{};
+  p.c = check_kv8(kc, vc, ks, vs, kt, vt);
+  c10::DeviceGuard g(kc.device());
+  check_kv8_qkv(qkv, p.c, kc, n_heads, n_kv_heads);
+  check_positions(pos, kc, p.c.B);
+  TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.is_contiguous() &&
+                  sin.is_contiguous() && cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.size(1) == p.c.D / 2 &&
+                  cos.size(0) >= p.c.Smax && cos.device() == kc.device() && sin.device() == kc.device(),
+              "kv8_append: rope tables must be contiguous fp32 [>= Smax, D / 2] on the cache's device");
+  check_align16(cos, "cos"); check_align16(sin, "sin");
+  no_overlap({&qkv, &kc, &vc, &ks, &vs, &kt, &vt});
+  const int64_t S = qkv.size(1);
+  TORCH_CHECK(S <= p.c.Smax, "kv8_append: ", S, " new tokens for a cache of ", p.c.Smax);
+  TORCH_CHECK(qkv.numel() / 8 < (int64_t(1) << 32) - (int64_t(1) << 24), "kv8_append: qkv too large for one launch");
+  p.qkv = qkv.data_ptr(); p.qkv_sb = qkv.stride(0); p.qkv_ss = qkv.stride(1);
+  p.pos = pos.data_ptr<int>(); p.cos = cos.data_ptr<float>(); p.sin = sin.data_ptr<float>();
+  p.S = (int)S; p.Hq = (int)n_heads;
+  dph::kv8_append(p, cur_stream());
+}
+
+Tensor kv8_decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+                            const Tensor& kt, const Tensor& vt, const Tensor& pos, int64_t n_heads, int64_t n_kv_heads,
+                            double scale, int64_t max_len) {
+  dph::KV8DecodeParams p{};
+  p.c = check_kv8(kc, vc, ks, vs, kt, vt);
+  c10::DeviceGuard g(kc.device());
+  check_kv8_qkv(qkv, p.c, kc, n_heads, n_kv_heads);
+  TORCH_CHECK(qkv.size(1) == 1, "kv8_decode_attention: one token per sequence (qkv [B, 1, ...])");
+  check_positions(pos, kc, p.c.B);
+  TORCH_CHECK(max_len >= 1 && max_len <= p.c.Smax, "kv8_decode_attention: max_len must be in [1, Smax]");
+  auto out = at::empty({p.c.B, n_heads * p.c.D}, qkv.options());
+  p.q = qkv.data_ptr(); p.q_sb = qkv.stride(0);
+  p.pos = pos.data_ptr<int>();
+  p.out = out.data_ptr();
+  p.Hq = (int)n_heads; p.scale = (float)scale;
+  dph::kv8_decode_attention(p, cur_stream());
+  return out;
+}
+
+void kv8_read_(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& kt,
+               const Tensor& vt, const Tensor& pos, Tensor& ko, Tensor& vo) {
+  dph::KV8ReadParams p{};
+  p.c = check_kv8(kc, vc, ks, vs, kt, vt);
+  c10::DeviceGuard g(kc.device());
+  check_positions(pos, kc, p.c.B);
+  TORCH_CHECK(ko.device() == kc.device() && vo.device() == kc.device() && ko.scalar_type() == at::kBFloat16 &&
+                  vo.scalar_type() == at::kBFloat16 && ko.dim() == 4 && ko.sizes() == vo.sizes() &&
+                  ko.strides() == vo.strides() && ko.size(0) == p.c.B && ko.size(2) == p.c.Hkv && ko.size(3) == p.c.D,
+              "kv8_read: outputs must be bf16 [B, count, Hkv, D] of equal strides on the cache's device");
+  TORCH_CHECK(ko.size(1) <= p.c.Smax, "kv8_read: count ", ko.size(1), " exceeds the cache's ", p.c.Smax, " rows");
+  TORCH_CHECK(strides_ok(ko, 8), "kv8_read: outputs need a contiguous head dim and strides that are multiples of 8");
+  check_align16(ko, "k_out"); check_align16(vo, "v_out");
+  no_overlap({&ko, &vo});
+  TORCH_CHECK(2 * ko.numel() / 8 < (int64_t(1) << 32) - 256, "kv8_read: too large for one launch");
+  p.pos = pos.data_ptr<int>();
+  p.ko = ko.data_ptr(); p.vo = vo.data_ptr(); p.o_sb = ko.stride(0); p.o_ss = ko.stride(1); p.o_sh = ko.stride(2);
+  p.count = (int)ko.size(1);
+  dph::kv8_read(p, cur_stream());
+}
+
+Tensor process_logits(const Tensor& logits, const c10::optional<Tensor>& tokens, const c10::optional<Tensor>& lengths,
+                      const c10::optional<Tensor>& prompt_lengths, const c10::optional<Tensor>& repetition,
+                      const c10::optional<Tensor>& presence, const c10::optional<Tensor>& frequency,
+                      const c10::optional<Tensor>& bias, const c10::optional<Tensor>& mask) {
+  check_cuda(logits, "logits");
+  c10::DeviceGuard g(logits.device());
+  TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+              "process_logits: logits must be [N, V] with a contiguous last dim");
+  const int64_t N = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V < (int64_t(1) << 31) - 8192 && N * (V / 1024 + 1) < (int64_t(1) << 24),
+              "process_logits: too many logits for one launch");
+  dph::LogitParams p{};
+  const int dt = dt_code(logits);
+  auto on = [&](const c10::optional<Tensor>& t, at::ScalarType st, const char* name) {
+    if (!t.has_value() || !t->defined()) return false;
+    TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == st, "process_logits: ", name, " must be ", st,
+                " on the device of the logits");
+    return true;
+  };
+  auto row = [&](const c10::optional<Tensor>& t, at::ScalarType st, const char* name) -> const void* {
+    if (!on(t, st, name)) return nullptr;
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == N && t->is_contiguous(), "process_logits: ", name, " must be [N]");
+    return t->data_ptr();
+  };
+  p.lengths = (const int*)row(lengths, at::kInt, "lengths");
+  p.prompt = (const int*)row(prompt_lengths, at::kInt, "prompt_lengths");
+  p.rep = (const float*)row(repetition, at::kFloat, "repetition");
+  p.pres = (const float*)row(presence, at::kFloat, "presence");
+  p.freq = (const float*)row(frequency, at::kFloat, "frequency");
+  if (on(tokens, at::kLong, "tokens")) {
+    TORCH_CHECK(tokens->dim() == 2 && tokens->size(0) == N && (tokens->size(1) <= 1 || tokens->stride(1) == 1) &&
+                    tokens->size(1) < (int64_t(1) << 31) - 8192,
+                "process_logits: tokens must be [N, L] with a contiguous last dim");
+    TORCH_CHECK(p.lengths, "process_logits: tokens need their lengths");
+    // without a penalty the history changes nothing
+    if (tokens->size(1) > 0 && (p.rep || p.pres || p.freq)) {
+      p.tokens = tokens->data_ptr<int64_t>(); p.ldt = tokens->stride(0); p.L = (int)tokens->size(1);
+    }
+  } else {
+    TORCH_CHECK(!p.lengths && !p.prompt && !p.rep && !p.pres && !p.freq,
+                "process_logits: lengths and penalties need tokens");
+  }
+  auto wide = [&](const c10::optional<Tensor>& t, at::ScalarType st, int64_t cols, const char* name, int64_t* ld)
+      -> const void* {
+    if (!on(t, st, name)) return nullptr;
+    TORCH_CHECK((t->dim() == 1 || (t->dim() == 2 && t->size(0) == N)) && t->size(-1) == cols &&
+                    (cols <= 1 || t->stride(-1) == 1), "process_logits: ", name, " must be [", cols, "] or [N, ", cols,
+                "] with a contiguous last dim");
+    *ld = t->dim() == 2 ? t->stride(0) : 0;
+    return t->data_ptr();
+  };
+  p.bias = (const float*)wide(bias, at::kFloat, V, "bias", &p.ldb);
+  p.mask = (const int*)wide(mask, at::kInt, (V + 31) / 32, "mask", &p.ldm);
+  auto y = at::empty({N, V}, logits.options());
+  p.x = logits.data_ptr(); p.ldx = logits.stride(0); p.y = y.data_ptr();
+  p.N = (int)N; p.V = (int)V;
+  dph::process_logits(p, dt, cur_stream());
+  return y;
 }
 
 Tensor skinny_linear(const Tensor& x, const Tensor& w) {
@@ -1736,6 +1917,15 @@ TORCH_LIBRARY(dph, m) {
         "int n_heads, int n_kv_heads, float kv_scale=1.) -> ()");
   m.def("decode_attention(Tensor qkv, Tensor k_cache, Tensor v_cache, Tensor pos, int n_heads, int n_kv_heads, "
         "float scale, int max_len, float kv_scale=1.) -> Tensor");
+  m.def("kv8_append_(Tensor(a!) qkv, Tensor(b!) k, Tensor(c!) v, Tensor(d!) k_scale, Tensor(e!) v_scale, "
+        "Tensor(f!) k_tail, Tensor(g!) v_tail, Tensor pos, Tensor cos, Tensor sin, int n_heads, int n_kv_heads) -> ()");
+  m.def("kv8_decode_attention(Tensor qkv, Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor k_tail, "
+        "Tensor v_tail, Tensor pos, int n_heads, int n_kv_heads, float scale, int max_len) -> Tensor");
+  m.def("kv8_read_(Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor k_tail, Tensor v_tail, Tensor pos, "
+        "Tensor(a!) k_out, Tensor(b!) v_out) -> ()");
+  m.def("process_logits(Tensor logits, Tensor? tokens=None, Tensor? lengths=None, Tensor? prompt_lengths=None, "
+        "Tensor? repetition=None, Tensor? presence=None, Tensor? frequency=None, Tensor? bias=None, "
+        "Tensor? mask=None) -> Tensor");
   m.def("skinny_linear(Tensor x, Tensor w) -> Tensor");
   m.def("gemv_swiglu(Tensor x2, Tensor w) -> Tensor");
   m.def("gemv_rmsnorm(Tensor x, Tensor? res, Tensor norm_weight, float eps, Tensor w) -> (Tensor, Tensor)");
@@ -1827,6 +2017,10 @@ TORCH_LIBRARY_IMPL(dph, CUDA, m) {
   m.impl("flash_attn_bwd_into", &flash_attn_bwd_into);
   m.impl("fp8_quantize", &fp8_quantize);
   m.impl("kv_append_", &kv_append_);
+  m.impl("kv8_append_", &kv8_append_);
+  m.impl("kv8_decode_attention", &kv8_decode_attention);
+  m.impl("kv8_read_", &kv8_read_);
+  m.impl("process_logits", &process_logits);
   m.impl("decode_attention", &decode_attention);
   m.impl("skinny_linear", &skinny_linear);
   m.impl("gemv_swiglu", &gemv_swiglu);

@@ -8,6 +8,8 @@ from .activations import GELU, gelu, swiglu, swiglu_reference
 from .batchnorm import BatchNormAct2d, batch_norm_act
 from .conv import Conv1x1, Conv3x3, StridedConv2d
 from .decode import decode_attention, kv_append_
+from .kv8 import KV8Cache, kv8_append_, kv8_cache, kv8_decode_attention, kv8_read
+from .logits import pack_token_mask, process_logits
 from .attention import attention_reference, flash_attention, flash_bwd, flash_fwd, rope_attention
 from .embedding import Embedding, embedding
 from .loss import fused_cross_entropy, latitude_weighted_mse, latitude_weights, vocab_parallel_cross_entropy
@@ -23,4 +25,5 @@ __all__ = [
     "latitude_weights", "vocab_parallel_cross_entropy", "LayerNorm", "RMSNorm", "add_rms_norm", "layer_norm",
     "rms_norm", "rmsnorm_reference", "apply_rope", "precompute_rope_tables", "rope_", "rope_reference",
     "native_available", "decode_attention", "kv_append_", "MaxPool2d", "max_pool2s2", "max_pool3s2",
+    "KV8Cache", "kv8_append_", "kv8_cache", "kv8_decode_attention", "kv8_read", "pack_token_mask", "process_logits",
 ]

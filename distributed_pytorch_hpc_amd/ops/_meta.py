@@ -314,6 +314,27 @@ def _decode_attention(qkv, k_cache, v_cache, pos, n_heads, n_kv_heads, scale, ma
     return qkv.new_empty((qkv.shape[0], n_heads * D))
 
 
+@register_fake("dph::kv8_append_")
+def _kv8_append(qkv, k, v, k_scale, v_scale, k_tail, v_tail, pos, cos, sin, n_heads, n_kv_heads):
+    return None
+
+
+@register_fake("dph::kv8_decode_attention")
+def _kv8_decode_attention(qkv, k, v, k_scale, v_scale, k_tail, v_tail, pos, n_heads, n_kv_heads, scale, max_len):
+    return qkv.new_empty((qkv.shape[0], n_heads * k.shape[-1]))
+
+
+@register_fake("dph::kv8_read_")
+def _kv8_read(k, v, k_scale, v_scale, k_tail, v_tail, pos, k_out, v_out):
+    return None
+
+
+@register_fake("dph::process_logits")
+def _process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repetition=None, presence=None,
+                    frequency=None, bias=None, mask=None):
+    return logits.new_empty(logits.shape)
+
+
 @register_fake("dph::skinny_linear")
 def _skinny_linear(x, w):
     return x.new_empty((*x.shape[:-1], w.shape[0]))
