@@ -380,7 +380,7 @@ struct KV8 {
   void* kc; void* vc; int64_t c_sb, c_ss, c_sh;      // codes [B, Smax, Hkv, D]
   float* ks; float* vs; int64_t s_sb, s_sn, s_sh;    // scales [B, Smax / T, Hkv]
   void* kt; void* vt; int64_t t_sb, t_ss, t_sh;      // open block, bf16 [B, T, Hkv, D]
-  int B, Smax, Hkv, D, T;
+  int B, Smax, Hkv, D, T, lgT;                       // T = 1 << lgT
   int e4m3;                                          // codes are OCP e4m3, else int8
 };
 struct KV8AppendParams {
@@ -397,7 +397,10 @@ struct KV8DecodeParams {
   void* out;                                         // bf16 [B, Hq * D]
   int Hq;
   float scale;
+  int chunk, units;                                  // keys of a unit of work, units that cover the longest sequence
+  float* opart; float* mlpart;                       // units > 1: workspace fp32 [B, Hq, units, D] / [B, Hq, units, 2]
 };
+int kv8_decode_chunk(int B, int Hkv, int Hq, int max_len);
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t stream);
 // rows pos[b] - count .. pos[b] - 1 of every sequence as bf16 [B, count, Hkv, D] (rows before the first token: zero)
 struct KV8ReadParams {

@@ -5,6 +5,9 @@
 //   scale = max(amax / QMAX, 2^-126),   code = round(x * (1 / scale)),   QMAX = 127 (int8) / 448 (e4m3)
 // and the block that is still open stays in bf16, so what the cache holds after n tokens does not depend on how they
 // were grouped into appends.  A block with an entry that is not finite gets the scale NaN and reads back as NaN.
+#include <algorithm>
+#include <type_traits>
+
 #include "dph_common.h"
 #include "kernels.h"
 
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
   const int pos = p.pos[b];
   if (pos < 0 || pos >= c.Smax) return;   // whole workgroup, before any barrier
   const int n = (int)min((int64_t)pos + p.S, (int64_t)c.Smax);
-  const int blk = pos / T + j, t0 = blk * T;
+  const int blk = (pos >> c.lgT) + j, t0 = blk * T;
   if (t0 >= n) return;
   const bool full = n - t0 >= T;
   if (!full && j > 0) return;
@@ -159,7 +162,7 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
     if (tid == 0) (is_k ? c.ks : c.vs)[(int64_t)b * c.s_sb + (int64_t)blk * c.s_sn + (int64_t)h * c.s_sh] = sc;
   }
   if (j == 0) {   // the barrier above ordered the tail's reads before these writes
-    const int o0 = n / T * T, from = max(o0, pos);
+    const int o0 = n >> c.lgT << c.lgT, from = max(o0, pos);
     for (int e = tid; e < (n - from) * CH; e += 256) {
       const int t = from + e / CH, ch = e % CH;
       *reinterpret_cast<bf16x8*>(tail + (int64_t)(t - o0) * c.t_ss + ch * 8) = fresh(t, ch);
@@ -170,10 +173,10 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
 // 8 elements of row t of the cache that holds n rows, in fp32
 template <bool E4M3>
 __device__ __forceinline__ void row8(const KV8& c, bool is_k, int b, int h, int t, int n, int ch, float (&o)[8]) {
-  if (t < n / c.T * c.T) {
+  if (t < n >> c.lgT << c.lgT) {
     const uint2 r = *reinterpret_cast<const uint2*>((const uint8_t*)(is_k ? c.kc : c.vc) + (int64_t)b * c.c_sb +
                                                     (int64_t)t * c.c_ss + (int64_t)h * c.c_sh + ch * 8);
-    const float sc = (is_k ? c.ks : c.vs)[(int64_t)b * c.s_sb + (int64_t)(t / c.T) * c.s_sn + (int64_t)h * c.s_sh];
+    const float sc = (is_k ? c.ks : c.vs)[(int64_t)b * c.s_sb + (int64_t)(t >> c.lgT) * c.s_sn + (int64_t)h * c.s_sh];
     float lo[4], hi[4];
     unpack4<E4M3>(r.x, lo);
     unpack4<E4M3>(r.y, hi);
@@ -183,56 +186,319 @@ __device__ __forceinline__ void row8(const KV8& c, bool is_k, int b, int h, int 
       o[4 + k] = hi[k] * sc;
     }
   } else {
-    Vec8<bf16>::load((const bf16*)(is_k ? c.kt : c.vt) + (int64_t)b * c.t_sb + (int64_t)(t % c.T) * c.t_ss +
+    Vec8<bf16>::load((const bf16*)(is_k ? c.kt : c.vt) + (int64_t)b * c.t_sb + (int64_t)(t & (c.T - 1)) * c.t_ss +
                          (int64_t)h * c.t_sh + ch * 8, o);
   }
 }
 
-// Decode attention, plain form: a workgroup per (sequence, query head), D / 8 lanes per key, online softmax per group
-// of lanes, groups and waves merged at the end.
-template <bool E4M3, int D>
-__global__ __launch_bounds__(256) void kv8_decode_k(KV8DecodeParams p) {
-  constexpr int CH = D / 8, GROUPS = 256 / CH;
-  __shared__ float sm[GROUPS], sl[GROUPS], so[GROUPS][D];
-  const KV8& c = p.c;
-  const int hq = blockIdx.x, b = blockIdx.y, h = hq / (p.Hq / c.Hkv);
-  const int g = threadIdx.x / CH, ch = threadIdx.x % CH;
-  const int n = max(0, min(p.pos[b], c.Smax - 1) + 1);
-  float q[8], acc[8] = {};
-  Vec8<bf16>::load((const bf16*)p.q + (int64_t)b * p.q_sb + (int64_t)hq * D + ch * 8, q);
-  float m = -INFINITY, l = 0.f;
-  for (int t = g; t < n; t += GROUPS) {
-    float k[8], v[8];
-    row8<E4M3>(c, true, b, h, t, n, ch, k);
-    row8<E4M3>(c, false, b, h, t, n, ch, v);
-    float s = 0.f;
+// ---- Decode attention: o = softmax(scale q K^T) V for one token of every sequence.
+//
+// Bound by the bytes of the codes: a key and value of one head are 2 D bytes, used by the G = Hq / Hkv query heads of
+// the group.  So a wave takes 32 keys at a time and ALL heads of the group (up to 16, the width of the matrix tile):
+//   S[key, head] = K q^T on v_mfma_f32_16x16x32_bf16, K as the A operand.  A code is exact in bf16 (8 significant bits
+//     at most), so the scales stay out of the products: S is multiplied by the block's scale in fp32.
+//   O^T[d, head] = V^T P, the accumulator of S reused as the B operand: a lane of S's result holds four keys of a head,
+//     which become its eight k-slots of two 16-key tiles, so P never leaves its lane.  V^T is the A operand under the same
+//     order of keys: lane (c, g) loads D / 16 contiguous bytes of its eight keys and takes byte e of each for d-tile e.
+//   The weights times the scale of V enter as the sum of two bf16 parts (16 significant bits) -- a second product over the
+//   operand that is converted anyway.
+// 8-bit -> bf16 conversion is the largest part of the arithmetic: about 1.5 instructions an element, a third of what the
+// vector units can do in the time that the bytes take.  Four waves of a workgroup share a unit of `chunk` keys in turns
+// of 32 and merge over LDS; where a sequence is longer than a unit, units leave unnormalised sums for kv8_combine_k.
+template <int D>
+struct Raw {   // the codes of one 32-key step in one lane
+  typedef typename std::conditional<D >= 64, u32x4, uint2>::type K;
+  typedef typename std::conditional<D == 128, uint2, typename std::conditional<D == 64, unsigned, uint16_t>::type>::type V;
+  K k[2][D >= 64 ? D / 64 : 1];
+  V v[8];
+  float ks[2], vs[2];
+};
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// four codes -> bf16, exact
+template <bool E4M3>
+__device__ __forceinline__ void widen4(unsigned r, bf16x8& o, int at) {
+  float f[4];
+  unpack4<E4M3>(r, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(q[e], k[e], s);
+  for (int j = 0; j < 4; ++j) o[at + j] = (bf16)f[j];
+}
+
+// byte e of eight values of 1, 2, 4 or 8 bytes
+__device__ __forceinline__ unsigned byte_of(uint2 v, int e) { return (e < 4 ? v.x >> (8 * e) : v.y >> (8 * (e - 4))) & 0xff; }
+__device__ __forceinline__ unsigned byte_of(unsigned v, int e) { return v >> (8 * e) & 0xff; }
+__device__ __forceinline__ unsigned byte_of(uint16_t v, int e) { return (unsigned)v >> (8 * e) & 0xff; }
+
+template <bool E4M3, typename V>
+__device__ __forceinline__ bf16x8 column(const V (&v)[8], int e) {
+  bf16x8 o;
+  if constexpr (E4M3) {
+    unsigned lo = 0, hi = 0;
 #pragma unroll
-    for (int o = CH / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    s *= p.scale * 1.4426950408889634f;
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-    const float a = exp2f(m - base), w = exp2f(s - base);
-    l = l * a + w;
+    for (int j = 0; j < 4; ++j) {
+      lo |= byte_of(v[j], e) << (8 * j);
+      hi |= byte_of(v[4 + j], e) << (8 * j);
+    }
+    widen4<true>(lo, o, 0);
+    widen4<true>(hi, o, 4);
+  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = acc[e] * a + w * v[e];
-    m = mn;   // a NaN score leaves m alone and makes l and acc NaN for good
+    for (int j = 0; j < 8; ++j) o[j] = (bf16)(float)(int8_t)byte_of(v[j], e);
   }
-  if (ch == 0) { sm[g] = m; sl[g] = l; }
+  return o;
+}
+
+// The running softmax of one wave: lane (c, g) holds head c's maximum, its own keys' share of the sum, and rows
+// (D / 16) (4 g + r) + e of O^T in acc[e][r].
+template <int D>
+struct Online {
+  f32x4 acc[D / 16];
+  float m, l;
+  __device__ __forceinline__ void init() {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) so[g][ch * 8 + e] = acc[e];
+    for (int e = 0; e < D / 16; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  // s: scores in units of log2 (-inf: no key); vs: scale of V of the two tiles; column(e): A operand of d-tile e
+  template <typename F>
+  __device__ __forceinline__ void step(const f32x4 (&s)[2], const float (&vs)[2], F&& vcol) {
+    float mx = m;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[a][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float base = mx == -INFINITY ? 0.f : mx;   // no key so far: exp2(-inf - 0) = 0
+    if (__any(mx > m)) {
+      const float a = exp2f(m - base);
+      l *= a;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) acc[e] *= a;
+    }
+    m = mx;
+    bf16x8 hi, lo;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = exp2f(s[a][r] - base);   // a NaN score leaves m alone and makes l and acc NaN for good
+        l += p;
+        const float w = p * vs[a];
+        const bf16 h = (bf16)w;
+        hi[4 * a + r] = h;
+        lo[4 * a + r] = (bf16)(w - (float)h);
+      }
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) {
+      const bf16x8 v = vcol(e);
+      acc[e] = mfma16(v, hi, acc[e]);
+      acc[e] = mfma16(v, lo, acc[e]);
+    }
+  }
+};
+
+template <bool E4M3, int D>
+__global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
+  constexpr int NI = D / 32, NE = D / 16, NH = D >= 64 ? D / 64 : 1, LD = D + 4;   // LD: rows of heads fall on other banks
+  __shared__ float so[4][16][LD];
+  __shared__ float sml[4][16][2];
+  const KV8& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
+  int id = blockIdx.x;
+  const int u = id % p.units;
+  id /= p.units;
+  const int G = p.Hq / c.Hkv, tiles = (G + 15) / 16;
+  const int ct = id % tiles;
+  id /= tiles;
+  const int h = id % c.Hkv, b = id / c.Hkv;
+  const int n = max(0, min(p.pos[b], c.Smax - 1) + 1);
+  const int lo = u * p.chunk, hi = min(n, lo + p.chunk);
+  const int hq0 = h * G + ct * 16, nq = min(16, G - ct * 16);
+  if (lo >= n) {   // no keys; a sequence without any has a zero output
+    if (n == 0 && u == 0)
+      for (int i = tid; i < nq * D; i += 256) ((bf16*)p.out)[((int64_t)b * p.Hq + hq0) * D + i] = (bf16)0.f;
+    return;
+  }
+  const int full = n >> c.lgT << c.lgT;
+  const float sl2 = p.scale * 1.4426950408889634f;
+
+  // q as the B operand: lane (head, g), chunk i holds the d that K's chunk i has in the lanes of group g
+  auto dof = [&](int i) { return D >= 64 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 8 * g; };
+  bf16x8 qf[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    qf[i] = bf16x8{};
+    if (r16 < nq)
+      qf[i] = *reinterpret_cast<const bf16x8*>((const bf16*)p.q + (int64_t)b * p.q_sb + (int64_t)(hq0 + r16) * D + dof(i));
+  }
+  Online<D> st;
+  st.init();
+
+  const uint8_t* kc = (const uint8_t*)c.kc + (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
+  const uint8_t* vc = (const uint8_t*)c.vc + (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
+  const float* ks = c.ks + (int64_t)b * c.s_sb + (int64_t)h * c.s_sh;
+  const float* vs = c.vs + (int64_t)b * c.s_sb + (int64_t)h * c.s_sh;
+  const int end = min(hi, full);   // keys lo .. end are codes; end - lo is a multiple of 16
+  auto load = [&](int k0, Raw<D>& w) {   // rows past the codes re-read the last one: their scores are masked
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const uint8_t* row = kc + (int64_t)min(k0 + 16 * a + r16, end - 1) * c.c_ss;
+#pragma unroll
+      for (int x = 0; x < NH; ++x)
+        w.k[a][x] = *reinterpret_cast<const typename Raw<D>::K*>(row + (D >= 64 ? 64 * x + 16 * g : 8 * g));
+      const int blk = __builtin_amdgcn_readfirstlane(min(k0 + 16 * a, end - 1) >> c.lgT);
+      w.ks[a] = ks[(int64_t)blk * c.s_sn];
+      w.vs[a] = vs[(int64_t)blk * c.s_sn];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w.v[j] = *reinterpret_cast<const typename Raw<D>::V*>(
+          vc + (int64_t)min(k0 + 16 * (j >> 2) + 4 * g + (j & 3), end - 1) * c.c_ss + r16 * (D / 16));
+  };
+  const int first = lo + 32 * wave;
+  if (first < end) {
+    Raw<D> cur, nxt;
+    load(first, cur);
+    for (int k0 = first; k0 < end; k0 += 128) {
+      load(k0 + 128 < end ? k0 + 128 : k0, nxt);   // the last turn re-reads its own keys: no branch around loads
+      f32x4 s[2];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          bf16x8 k;
+          if constexpr (D >= 64) {
+            widen4<E4M3>(cur.k[a][i >> 1][2 * (i & 1)], k, 0);
+            widen4<E4M3>(cur.k[a][i >> 1][2 * (i & 1) + 1], k, 4);
+          } else {
+            widen4<E4M3>(cur.k[a][0].x, k, 0);
+            widen4<E4M3>(cur.k[a][0].y, k, 4);
+          }
+          s[a] = mfma16(k, qf[i], s[a]);
+        }
+        const float f = sl2 * cur.ks[a];
+        const bool there = k0 + 16 * a < end;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[a][r] = there ? s[a][r] * f : -INFINITY;
+      }
+      st.step(s, cur.vs, [&](int e) { return column<E4M3>(cur.v, e); });
+      cur = nxt;
+    }
+  }
+  // the open block's bf16 rows, 32 of them a wave
+  const int t0 = 32 * wave, rows = hi - full;
+  if (t0 < rows) {
+    const bf16* kt = (const bf16*)c.kt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
+    const bf16* vt = (const bf16*)c.vt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
+    f32x4 s[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const bf16* row = kt + (int64_t)min(t0 + 16 * a + r16, rows - 1) * c.t_ss;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) s[a] = mfma16(*reinterpret_cast<const bf16x8*>(row + dof(i)), qf[i], s[a]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[a][r] = t0 + 16 * a + 4 * g + r < rows ? s[a][r] * sl2 : -INFINITY;
+    }
+    typedef __bf16 vrow __attribute__((ext_vector_type(NE)));
+    vrow v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = *reinterpret_cast<const vrow*>(vt + (int64_t)min(t0 + 16 * (j >> 2) + 4 * g + (j & 3), rows - 1) * c.t_ss +
+                                            r16 * NE);
+    const float one[2] = {1.f, 1.f};
+    st.step(s, one, [&](int e) {
+      bf16x8 o;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = v[j][e];
+      return o;
+    });
+  }
+
+  // merge the four waves
+  float l = st.l;
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (r16 < nq) {
+    if (g == 0) {
+      sml[wave][r16][0] = st.m;
+      sml[wave][r16][1] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) so[wave][r16][NE * (4 * g + r) + e] = st.acc[e][r];
+  }
+  __syncthreads();
+  for (int i = tid; i < nq * D; i += 256) {
+    const int q = i / D, d = i % D;
+    float M = -INFINITY, L = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, sml[w][q][0]);
+    const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float a = exp2f(sml[w][q][0] - base);
+      L = fmaf(a, sml[w][q][1], L);
+      o = fmaf(a, so[w][q][d], o);
+    }
+    const int64_t row = (int64_t)b * p.Hq + hq0 + q;
+    if (p.units == 1) {
+      ((bf16*)p.out)[row * D + d] = (bf16)(o / L);
+    } else {
+      const int64_t slot = row * p.units + u;
+      p.opart[slot * D + d] = o;
+      if (d == 0) {
+        p.mlpart[2 * slot] = M;
+        p.mlpart[2 * slot + 1] = L;
+      }
+    }
+  }
+}
+
+// One workgroup per (sequence, query head): its waves take the units in turns, then merge.  D / 64 (at least 1) elements a
+// lane.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_combine_k(KV8DecodeParams p) {
+  constexpr int E = D >= 64 ? D / 64 : 1;
+  __shared__ float so[4][D], sl[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const int n = max(0, min(p.pos[row / p.Hq], p.c.Smax - 1) + 1), nu = min((int)cdiv(n, p.chunk), p.units);
+  if (nu == 0) return;   // zeros already stored
+  const float* ml = p.mlpart + row * p.units * 2;
+  const float* op = p.opart + row * p.units * D;
+  float M = -INFINITY;
+  for (int i = lane; i < nu; i += 64) M = fmaxf(M, ml[2 * i]);
+  M = wave_max(M);
+  const float base = M == -INFINITY ? 0.f : M;
+  const bool active = lane * E < D;
+  float L = 0.f, o[E] = {};
+#pragma unroll 4
+  for (int i = wave; i < nu; i += 4) {
+    const float a = exp2f(ml[2 * i] - base);
+    L = fmaf(a, ml[2 * i + 1], L);
+    if (active) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(a, op[(int64_t)i * D + lane * E + e], o[e]);
+    }
+  }
+  if (lane == 0) sl[wave] = L;
+  if (active) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
+  }
   __syncthreads();
   if ((int)threadIdx.x < D) {
-    float M = -INFINITY;
-    for (int i = 0; i < GROUPS; ++i) M = fmaxf(M, sm[i]);
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f, o = 0.f;
-    for (int i = 0; i < GROUPS; ++i) {
-      const float w = exp2f(sm[i] - base);
-      L += w * sl[i];
-      o += w * so[i][threadIdx.x];
-    }
-    ((bf16*)p.out)[(int64_t)b * p.Hq * D + hq * D + threadIdx.x] = (bf16)(n > 0 ? o / L : 0.f);
+    const int d = threadIdx.x;
+    const float sum = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]), all = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    ((bf16*)p.out)[row * D + d] = (bf16)(sum / all);
   }
 }
 
@@ -281,16 +547,26 @@ void kv8_append(const KV8AppendParams& p, hipStream_t st) {
 #undef DPH_KV8_APP
 }
 
+// Keys of one unit of work: enough units to fill the card several times over whatever the batch (ragged sequences then
+// even out), no fewer than a step of each wave, and a multiple of every block size, so that no open block crosses units.
+int kv8_decode_chunk(int B, int Hkv, int Hq, int max_len) {
+  const int64_t rows = (int64_t)B * Hkv * cdiv(Hq / Hkv, 16);
+  const int64_t keys = cdiv(rows * max_len, 1024);
+  return (int)(128 * std::max<int64_t>(1, cdiv(keys, 128)));
+}
+
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.Hq, (unsigned)p.c.B);
-  if (p.c.B == 0) return;
+  const KV8& c = p.c;
+  if (c.B == 0) return;
+  const dim3 grid((unsigned)((int64_t)p.units * c.B * c.Hkv * cdiv(p.Hq / c.Hkv, 16)));
 #define DPH_KV8_DEC(D_)                                                                          \
   do {                                                                                           \
-    if (p.c.e4m3) hipLaunchKernelGGL((kv8_decode_k<true, D_>), grid, dim3(256), 0, st, p);       \
+    if (c.e4m3) hipLaunchKernelGGL((kv8_decode_k<true, D_>), grid, dim3(256), 0, st, p);         \
     else hipLaunchKernelGGL((kv8_decode_k<false, D_>), grid, dim3(256), 0, st, p);               \
+    if (p.units > 1) hipLaunchKernelGGL(kv8_combine_k<D_>, dim3((unsigned)(c.B * p.Hq)), dim3(256), 0, st, p); \
   } while (0)
-  if (p.c.D == 128) DPH_KV8_DEC(128);
-  else if (p.c.D == 64) DPH_KV8_DEC(64);
+  if (c.D == 128) DPH_KV8_DEC(128);
+  else if (c.D == 64) DPH_KV8_DEC(64);
   else DPH_KV8_DEC(32);
 #undef DPH_KV8_DEC
 }

@@ -542,7 +542,7 @@ dph::KV8 check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const T
   c.ks = ks.data_ptr<float>(); c.vs = vs.data_ptr<float>();
   c.s_sb = ks.stride(0); c.s_sn = ks.stride(1); c.s_sh = ks.stride(2);
   c.kt = kt.data_ptr(); c.vt = vt.data_ptr(); c.t_sb = kt.stride(0); c.t_ss = kt.stride(1); c.t_sh = kt.stride(2);
-  c.B = (int)B; c.Smax = (int)Smax; c.Hkv = (int)H; c.D = (int)D; c.T = (int)T; c.e4m3 = e4m3 ? 1 : 0;
+  c.B = (int)B; c.Smax = (int)Smax; c.Hkv = (int)H; c.D = (int)D; c.T = (int)T; c.lgT = __builtin_ctz((unsigned)T); c.e4m3 = e4m3 ? 1 : 0;
   return c;
 }
 
@@ -600,6 +600,14 @@ Tensor kv8_decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& v
   p.pos = pos.data_ptr<int>();
   p.out = out.data_ptr();
   p.Hq = (int)n_heads; p.scale = (float)scale;
+  p.chunk = dph::kv8_decode_chunk(p.c.B, p.c.Hkv, p.Hq, (int)max_len);
+  p.units = (int)((max_len + p.chunk - 1) / p.chunk);
+  Tensor opart, ml;
+  if (p.units > 1) {
+    opart = at::empty({p.c.B, n_heads, p.units, p.c.D}, qkv.options().dtype(at::kFloat));
+    ml = at::empty({p.c.B, n_heads, p.units, 2}, qkv.options().dtype(at::kFloat));
+    p.opart = opart.data_ptr<float>(); p.mlpart = ml.data_ptr<float>();
+  }
   dph::kv8_decode_attention(p, cur_stream());
   return out;
 }
