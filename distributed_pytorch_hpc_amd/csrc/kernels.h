@@ -400,7 +400,7 @@ struct KV8DecodeParams {
   int chunk, units;                                  // keys of a unit of work, units that cover the longest sequence
   float* opart; float* mlpart;                       // units > 1: workspace fp32 [B, Hq, units, D] / [B, Hq, units, 2]
 };
-int kv8_decode_chunk(int B, int Hkv, int Hq, int max_len);
+int kv8_decode_chunk(int B, int Hkv, int Hq, int T, int max_len);
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t stream);
 // rows pos[b] - count .. pos[b] - 1 of every sequence as bf16 [B, count, Hkv, D] (rows before the first token: zero)
 struct KV8ReadParams {

@@ -37,6 +37,9 @@ __device__ __forceinline__ unsigned pack4(const float (&q)[4]) {
   }
 }
 
+// byte e, signed: shifts of 32 bits fold into a conversion that selects the byte, those of a narrower type do not
+__device__ __forceinline__ int sbyte_of(unsigned v, int e) { return (int)(v << (24 - 8 * e)) >> 24; }
+
 template <bool E4M3>
 __device__ __forceinline__ void unpack4(unsigned r, float (&o)[4]) {
   if constexpr (E4M3) {
@@ -44,7 +47,7 @@ __device__ __forceinline__ void unpack4(unsigned r, float (&o)[4]) {
     o[0] = a[0]; o[1] = a[1]; o[2] = b[0]; o[3] = b[1];
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = (float)(int8_t)(r >> (8 * j));
+    for (int j = 0; j < 4; ++j) o[j] = (float)sbyte_of(r, j);
   }
 }
 
@@ -206,12 +209,9 @@ __device__ __forceinline__ void row8(const KV8& c, bool is_k, int b, int h, int 
 // vector units can do in the time that the bytes take.  Four waves of a workgroup share a unit of `chunk` keys in turns
 // of 32 and merge over LDS; where a sequence is longer than a unit, units leave unnormalised sums for kv8_combine_k.
 template <int D>
-struct Raw {   // the codes of one 32-key step in one lane
+struct Raw {   // a lane's share of the codes of one key (K) and of one key's part of a head (V)
   typedef typename std::conditional<D >= 64, u32x4, uint2>::type K;
   typedef typename std::conditional<D == 128, uint2, typename std::conditional<D == 64, unsigned, uint16_t>::type>::type V;
-  K k[2][D >= 64 ? D / 64 : 1];
-  V v[8];
-  float ks[2], vs[2];
 };
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -232,6 +232,8 @@ __device__ __forceinline__ unsigned byte_of(uint2 v, int e) { return (e < 4 ? v.
 __device__ __forceinline__ unsigned byte_of(unsigned v, int e) { return v >> (8 * e) & 0xff; }
 __device__ __forceinline__ unsigned byte_of(uint16_t v, int e) { return (unsigned)v >> (8 * e) & 0xff; }
 
+__device__ __forceinline__ int sbyte_of(uint2 v, int e) { return sbyte_of(e < 4 ? v.x : v.y, e & 3); }
+
 template <bool E4M3, typename V>
 __device__ __forceinline__ bf16x8 column(const V (&v)[8], int e) {
   bf16x8 o;
@@ -246,10 +248,13 @@ __device__ __forceinline__ bf16x8 column(const V (&v)[8], int e) {
     widen4<true>(hi, o, 4);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = (bf16)(float)(int8_t)byte_of(v[j], e);
+    for (int j = 0; j < 8; ++j) o[j] = (bf16)(float)sbyte_of(v[j], e);
   }
   return o;
 }
+
+// 2^x, zero below 2^-126: a weight that small adds nothing
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The running softmax of one wave: lane (c, g) holds head c's maximum, its own keys' share of the sum, and rows
 // (D / 16) (4 g + r) + e of O^T in acc[e][r].
@@ -275,7 +280,7 @@ struct Online {
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     const float base = mx == -INFINITY ? 0.f : mx;   // no key so far: exp2(-inf - 0) = 0
     if (__any(mx > m)) {
-      const float a = exp2f(m - base);
+      const float a = fast_exp2(m - base);
       l *= a;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) acc[e] *= a;
@@ -286,7 +291,7 @@ struct Online {
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = exp2f(s[a][r] - base);   // a NaN score leaves m alone and makes l and acc NaN for good
+        const float p = fast_exp2(s[a][r] - base);   // a NaN score leaves m alone and makes l and acc NaN for good
         l += p;
         const float w = p * vs[a];
         const bf16 h = (bf16)w;
@@ -303,7 +308,7 @@ struct Online {
 };
 
 template <bool E4M3, int D>
-__global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
+__global__ __launch_bounds__(256, 4) void kv8_decode_k(KV8DecodeParams p) {
   constexpr int NI = D / 32, NE = D / 16, NH = D >= 64 ? D / 64 : 1, LD = D + 4;   // LD: rows of heads fall on other banks
   __shared__ float so[4][16][LD];
   __shared__ float sml[4][16][2];
@@ -339,56 +344,70 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
   Online<D> st;
   st.init();
 
-  const uint8_t* kc = (const uint8_t*)c.kc + (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
-  const uint8_t* vc = (const uint8_t*)c.vc + (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
-  const float* ks = c.ks + (int64_t)b * c.s_sb + (int64_t)h * c.s_sh;
-  const float* vs = c.vs + (int64_t)b * c.s_sb + (int64_t)h * c.s_sh;
   const int end = min(hi, full);   // keys lo .. end are codes; end - lo is a multiple of 16
-  auto load = [&](int k0, Raw<D>& w) {   // rows past the codes re-read the last one: their scores are masked
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const uint8_t* row = kc + (int64_t)min(k0 + 16 * a + r16, end - 1) * c.c_ss;
-#pragma unroll
-      for (int x = 0; x < NH; ++x)
-        w.k[a][x] = *reinterpret_cast<const typename Raw<D>::K*>(row + (D >= 64 ? 64 * x + 16 * g : 8 * g));
-      const int blk = __builtin_amdgcn_readfirstlane(min(k0 + 16 * a, end - 1) >> c.lgT);
-      w.ks[a] = ks[(int64_t)blk * c.s_sn];
-      w.vs[a] = vs[(int64_t)blk * c.s_sn];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      w.v[j] = *reinterpret_cast<const typename Raw<D>::V*>(
-          vc + (int64_t)min(k0 + 16 * (j >> 2) + 4 * g + (j & 3), end - 1) * c.c_ss + r16 * (D / 16));
-  };
-  const int first = lo + 32 * wave;
+  const int first = lo + 32 * __builtin_amdgcn_readfirstlane(wave);
   if (first < end) {
-    Raw<D> cur, nxt;
-    load(first, cur);
+    // lane i keeps the scales of the unit's block i (chunk <= 64 T): no load of a single float inside the loop
+    const int blk0 = lo >> c.lgT;
+    float ksl = 0.f, vsl = 0.f;
+    if (lane < (end - lo) >> c.lgT) {
+      const int64_t at = (int64_t)b * c.s_sb + (int64_t)h * c.s_sh + (int64_t)(blk0 + lane) * c.s_sn;
+      ksl = c.ks[at];
+      vsl = c.vs[at];
+    }
+    auto scale_at = [&](float v, int key) {
+      return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), (key >> c.lgT) - blk0));
+    };
+    // uniform base of a 16-key tile plus 32-bit offsets of the lane that stay the same; where the codes end with the
+    // step's first tile (T = 16), the second one re-reads it and is masked
+    const int64_t head = (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
+    const int ss = (int)c.c_ss;
+    const unsigned ko = (unsigned)(r16 * ss + (D >= 64 ? 16 : 8) * g);
+    unsigned vo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vo[j] = (unsigned)((4 * g + j) * ss + r16 * NE);
+    auto tile = [&](int k0, int a) { return head + (int64_t)(k0 + (a && k0 + 16 < end ? 16 : 0)) * c.c_ss; };
+    typename Raw<D>::K k[2][NH];
+    auto load_k = [&](int k0) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const uint8_t* base = (const uint8_t*)c.kc + tile(k0, a);
+#pragma unroll
+        for (int x = 0; x < NH; ++x) k[a][x] = *reinterpret_cast<const typename Raw<D>::K*>(base + ko + 64 * x);
+      }
+    };
+    load_k(first);
     for (int k0 = first; k0 < end; k0 += 128) {
-      load(k0 + 128 < end ? k0 + 128 : k0, nxt);   // the last turn re-reads its own keys: no branch around loads
+      typename Raw<D>::V v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = *reinterpret_cast<const typename Raw<D>::V*>((const uint8_t*)c.vc + tile(k0, j >> 2) + vo[j & 3]);
       f32x4 s[2];
+      float vs[2];
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          bf16x8 k;
+          bf16x8 kb;
           if constexpr (D >= 64) {
-            widen4<E4M3>(cur.k[a][i >> 1][2 * (i & 1)], k, 0);
-            widen4<E4M3>(cur.k[a][i >> 1][2 * (i & 1) + 1], k, 4);
+            widen4<E4M3>(k[a][i >> 1][2 * (i & 1)], kb, 0);
+            widen4<E4M3>(k[a][i >> 1][2 * (i & 1) + 1], kb, 4);
           } else {
-            widen4<E4M3>(cur.k[a][0].x, k, 0);
-            widen4<E4M3>(cur.k[a][0].y, k, 4);
+            widen4<E4M3>(k[a][0].x, kb, 0);
+            widen4<E4M3>(k[a][0].y, kb, 4);
           }
-          s[a] = mfma16(k, qf[i], s[a]);
+          s[a] = mfma16(kb, qf[i], s[a]);
         }
-        const float f = sl2 * cur.ks[a];
-        const bool there = k0 + 16 * a < end;
+        const int key = a && k0 + 16 < end ? k0 + 16 : k0;
+        const float f = sl2 * scale_at(ksl, key);
+        vs[a] = scale_at(vsl, key);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[a][r] = there ? s[a][r] * f : -INFINITY;
+        for (int r = 0; r < 4; ++r) s[a][r] *= f;
       }
-      st.step(s, cur.vs, [&](int e) { return column<E4M3>(cur.v, e); });
-      cur = nxt;
+      if (k0 + 16 >= end) s[1] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      load_k(k0 + 128 < end ? k0 + 128 : k0);   // the last turn re-reads its own keys: no branch around loads
+      st.step(s, vs, [&](int e) { return column<E4M3>(v, e); });
     }
   }
   // the open block's bf16 rows, 32 of them a wave
@@ -444,7 +463,7 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
     const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float a = exp2f(sml[w][q][0] - base);
+      const float a = fast_exp2(sml[w][q][0] - base);
       L = fmaf(a, sml[w][q][1], L);
       o = fmaf(a, so[w][q][d], o);
     }
@@ -482,7 +501,7 @@ __global__ __launch_bounds__(256) void kv8_combine_k(KV8DecodeParams p) {
   float L = 0.f, o[E] = {};
 #pragma unroll 4
   for (int i = wave; i < nu; i += 4) {
-    const float a = exp2f(ml[2 * i] - base);
+    const float a = fast_exp2(ml[2 * i] - base);
     L = fmaf(a, ml[2 * i + 1], L);
     if (active) {
 #pragma unroll
@@ -549,10 +568,10 @@ void kv8_append(const KV8AppendParams& p, hipStream_t st) {
 
 // Keys of one unit of work: enough units to fill the card several times over whatever the batch (ragged sequences then
 // even out), no fewer than a step of each wave, and a multiple of every block size, so that no open block crosses units.
-int kv8_decode_chunk(int B, int Hkv, int Hq, int max_len) {
+int kv8_decode_chunk(int B, int Hkv, int Hq, int T, int max_len) {
   const int64_t rows = (int64_t)B * Hkv * cdiv(Hq / Hkv, 16);
   const int64_t keys = cdiv(rows * max_len, 1024);
-  return (int)(128 * std::max<int64_t>(1, cdiv(keys, 128)));
+  return (int)std::min<int64_t>(128 * std::max<int64_t>(1, cdiv(keys, 128)), 64 * T);   // a lane holds a block's scales
 }
 
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t st) {

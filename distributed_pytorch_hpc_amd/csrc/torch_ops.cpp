@@ -536,6 +536,7 @@ dph::KV8 check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const T
               "kv8: scales [B, Smax / T, Hkv] and tails [B, T, Hkv, D] must match k / v [B, Smax, Hkv, D]");
   TORCH_CHECK(strides_ok(kc, 16) && strides_ok(kt, 8),
               "kv8: head dim contiguous, the other strides multiples of 16 bytes");
+  TORCH_CHECK(kc.stride(1) >= 0 && kc.stride(1) < (int64_t(1) << 26), "kv8: rows of k / v more than 64 MB apart");
   check_align16(kc, "k"); check_align16(vc, "v"); check_align16(kt, "k_tail"); check_align16(vt, "v_tail");
   dph::KV8 c{};
   c.kc = kc.data_ptr(); c.vc = vc.data_ptr(); c.c_sb = kc.stride(0); c.c_ss = kc.stride(1); c.c_sh = kc.stride(2);
@@ -600,7 +601,7 @@ Tensor kv8_decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& v
   p.pos = pos.data_ptr<int>();
   p.out = out.data_ptr();
   p.Hq = (int)n_heads; p.scale = (float)scale;
-  p.chunk = dph::kv8_decode_chunk(p.c.B, p.c.Hkv, p.Hq, (int)max_len);
+  p.chunk = dph::kv8_decode_chunk(p.c.B, p.c.Hkv, p.Hq, p.c.T, (int)max_len);
   p.units = (int)((max_len + p.chunk - 1) / p.chunk);
   Tensor opart, ml;
   if (p.units > 1) {
