@@ -397,10 +397,12 @@ struct KV8DecodeParams {
   void* out;                                         // bf16 [B, Hq * D]
   int Hq;
   float scale;
-  int chunk, units;                                  // keys of a unit of work, units that cover the longest sequence
-  float* opart; float* mlpart;                       // units > 1: workspace fp32 [B, Hq, units, D] / [B, Hq, units, 2]
+  int wgs, tiles;                                    // workgroups; tiles of 16 query heads in a group, ceil(Hq / Hkv / 16)
+  float* opart; float* mlpart; int* info;            // workspace: sums and (max, sum) of shared rows, fp32 [wgs, 2, 16, D]
+                                                     // and [wgs, 2, 16, 2], and int32 [B, Hkv, tiles, 2] who shares a
+                                                     // row; null where max_len <= 128: no row is shared then
 };
-int kv8_decode_chunk(int B, int Hkv, int Hq, int T, int max_len);
+int kv8_decode_workgroups(int64_t turns);            // turns: B * Hkv * tiles * ceil(max_len / 128)
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t stream);
 // rows pos[b] - count .. pos[b] - 1 of every sequence as bf16 [B, count, Hkv, D] (rows before the first token: zero)
 struct KV8ReadParams {

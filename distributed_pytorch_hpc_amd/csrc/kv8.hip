@@ -206,8 +206,8 @@ __device__ __forceinline__ void row8(const KV8& c, bool is_k, int b, int h, int 
 //   The weights times the scale of V enter as the sum of two bf16 parts (16 significant bits) -- a second product over the
 //   operand that is converted anyway.
 // 8-bit -> bf16 conversion is the largest part of the arithmetic: about 1.5 instructions an element, a third of what the
-// vector units can do in the time that the bytes take.  Four waves of a workgroup share a unit of `chunk` keys in turns
-// of 32 and merge over LDS; where a sequence is longer than a unit, units leave unnormalised sums for kv8_combine_k.
+// vector units can do in the time that the bytes take.  Four waves of a workgroup share a turn of 128 keys and merge over
+// LDS; where several workgroups share a row, they leave unnormalised sums for kv8_combine_k.
 template <int D>
 struct Raw {   // a lane's share of the codes of one key (K) and of one key's part of a head (V)
   typedef typename std::conditional<D >= 64, u32x4, uint2>::type K;
@@ -307,208 +307,311 @@ struct Online {
   }
 };
 
+// The work of a call, in turns of 128 keys (32 for each wave of a workgroup): row (b, h, tile of 16 heads) has
+// ceil(n_b / 128) turns, at least one, and the rows' turns stand in one line, which the workgroups divide evenly whatever
+// the lengths are -- with a fixed number of keys a workgroup, sequences of 1000 to 4000 tokens left the card half idle at
+// the end (73 us against 5.5 TB/s at equal lengths).  The lengths are only known on the device, so every workgroup adds
+// them up for itself.
+struct Line {
+  int turns;       // of all rows
+  int per, rem;    // workgroup w has per + (w < rem) of them, from share_of(w)
+  int b, n, row0;  // the sequence of this workgroup's first turn, its length, and the turn at which its rows begin
+};
+
+__device__ __forceinline__ int length_of(const KV8DecodeParams& p, int b) {
+  return max(0, min(p.pos[b], p.c.Smax - 1) + 1);
+}
+// turns that a row of n keys counts for; one, where there is no workspace for shares of it (max_len <= 128)
+__device__ __forceinline__ int turns_of(const KV8DecodeParams& p, int n) { return p.opart ? max(1, (n + 127) >> 7) : 1; }
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// workgroups past the last turn (fewer turns than workgroups) begin and end there
+__device__ __forceinline__ int share_of(const Line& o, int w) { return min(w * o.per + min(w, o.rem), o.turns); }
+__device__ __forceinline__ int owner_of(const Line& o, int turn) {
+  const int big = o.rem * (o.per + 1);
+  return turn < big ? (unsigned)turn / (unsigned)(o.per + 1) : o.rem + (unsigned)(turn - big) / (unsigned)o.per;
+}
+
+// inclusive sum over the wave's lanes: within rows of 16 lanes, then across them (DPP: no trip through LDS)
+__device__ __forceinline__ int scan64(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast 31 into rows 2 and 3
+  return v;
+}
+
+__device__ __forceinline__ Line line_up(const KV8DecodeParams& p, int w) {
+  const int lane = threadIdx.x & 63, B = p.c.B, heads = p.c.Hkv * p.tiles;
+  Line o;
+  int total = 0, scan = 0, nt = 0, n = 0;
+  auto sum_up = [&](int base) {
+    n = base + lane < B ? length_of(p, base + lane) : 0;
+    nt = base + lane < B ? turns_of(p, n) : 0;
+    scan = scan64(nt);
+  };
+  for (int base = 0; base < B; base += 64) {
+    sum_up(base);
+    total += __builtin_amdgcn_readlane(scan, 63);
+  }
+  o.turns = total * heads;
+  const int wgs = min(p.wgs, o.turns);
+  o.per = uni((unsigned)o.turns / (unsigned)wgs);
+  o.rem = o.turns - o.per * wgs;
+  const int at = share_of(o, w);
+  o.b = o.n = o.row0 = 0;
+  for (int base = 0, before = 0; base < B; base += 64) {
+    if (B > 64) sum_up(base);   // otherwise the sums above still stand
+    const unsigned long long hit = __ballot((before + scan) * heads > at);
+    if (hit) {
+      const int l = uni(__ffsll(hit) - 1);
+      o.b = base + l;
+      o.n = __builtin_amdgcn_readlane(n, l);
+      o.row0 = (before + __builtin_amdgcn_readlane(scan - nt, l)) * heads;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(scan, 63);
+  }
+  return o;
+}
+
 template <bool E4M3, int D>
-__global__ __launch_bounds__(256, 4) void kv8_decode_k(KV8DecodeParams p) {
+__global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
   constexpr int NI = D / 32, NE = D / 16, NH = D >= 64 ? D / 64 : 1, LD = D + 4;   // LD: rows of heads fall on other banks
   __shared__ float so[4][16][LD];
   __shared__ float sml[4][16][2];
   const KV8& c = p.c;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
-  int id = blockIdx.x;
-  const int u = id % p.units;
-  id /= p.units;
-  const int G = p.Hq / c.Hkv, tiles = (G + 15) / 16;
-  const int ct = id % tiles;
-  id /= tiles;
-  const int h = id % c.Hkv, b = id / c.Hkv;
-  const int n = max(0, min(p.pos[b], c.Smax - 1) + 1);
-  const int lo = u * p.chunk, hi = min(n, lo + p.chunk);
-  const int hq0 = h * G + ct * 16, nq = min(16, G - ct * 16);
-  if (lo >= n) {   // no keys; a sequence without any has a zero output
-    if (n == 0 && u == 0)
-      for (int i = tid; i < nq * D; i += 256) ((bf16*)p.out)[((int64_t)b * p.Hq + hq0) * D + i] = (bf16)0.f;
-    return;
-  }
-  const int full = n >> c.lgT << c.lgT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), r16 = lane & 15, g = lane >> 4;
+  const int w = blockIdx.x, G = p.Hq / c.Hkv, heads = c.Hkv * p.tiles;
+  const Line line = line_up(p, w);
+  int at = share_of(line, w);
+  const int stop = share_of(line, w + 1);
+  if (at >= stop) return;
+  int b = line.b, n = line.n, nt = turns_of(p, n);
+  int row = uni((unsigned)(at - line.row0) / (unsigned)nt), t0 = at - line.row0 - row * nt;
   const float sl2 = p.scale * 1.4426950408889634f;
-
-  // q as the B operand: lane (head, g), chunk i holds the d that K's chunk i has in the lanes of group g
+  // the d of chunk i of a key (and so of q) in the lanes of group g
   auto dof = [&](int i) { return D >= 64 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 8 * g; };
-  bf16x8 qf[NI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    qf[i] = bf16x8{};
-    if (r16 < nq)
-      qf[i] = *reinterpret_cast<const bf16x8*>((const bf16*)p.q + (int64_t)b * p.q_sb + (int64_t)(hq0 + r16) * D + dof(i));
-  }
-  Online<D> st;
-  st.init();
 
-  const int end = min(hi, full);   // keys lo .. end are codes; end - lo is a multiple of 16
-  const int first = lo + 32 * __builtin_amdgcn_readfirstlane(wave);
-  if (first < end) {
-    // lane i keeps the scales of the unit's block i (chunk <= 64 T): no load of a single float inside the loop
-    const int blk0 = lo >> c.lgT;
-    float ksl = 0.f, vsl = 0.f;
-    if (lane < (end - lo) >> c.lgT) {
-      const int64_t at = (int64_t)b * c.s_sb + (int64_t)h * c.s_sh + (int64_t)(blk0 + lane) * c.s_sn;
-      ksl = c.ks[at];
-      vsl = c.vs[at];
+  while (true) {   // one row's share of this workgroup's turns at a time: t0 .. t1 of nt
+    const int t1 = min(nt, t0 + stop - at);
+    const int h = p.tiles == 1 ? row : uni((unsigned)row / (unsigned)p.tiles), ct = row - h * p.tiles;
+    const int hq0 = h * G + ct * 16, nq = min(16, G - ct * 16);
+    const int full = n >> c.lgT << c.lgT;
+    bf16x8 qf[NI];   // q as the B operand: lane (head, g)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      qf[i] = bf16x8{};
+      if (r16 < nq)
+        qf[i] = *reinterpret_cast<const bf16x8*>((const bf16*)p.q + (int64_t)b * p.q_sb + (int64_t)(hq0 + r16) * D + dof(i));
     }
-    auto scale_at = [&](float v, int key) {
-      return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), (key >> c.lgT) - blk0));
-    };
-    // uniform base of a 16-key tile plus 32-bit offsets of the lane that stay the same; where the codes end with the
-    // step's first tile (T = 16), the second one re-reads it and is masked
-    const int64_t head = (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
-    const int ss = (int)c.c_ss;
-    const unsigned ko = (unsigned)(r16 * ss + (D >= 64 ? 16 : 8) * g);
-    unsigned vo[4];
+    Online<D> st;
+    st.init();
+
+    const int end = t1 == nt ? full : 128 * t1;   // keys 128 t0 .. end are codes; a multiple of 16
+    const int first = 128 * t0 + 32 * wave;
+    if (first < end) {
+      // spans of 64 blocks: lane i keeps the scales of the span's block i, so the loop over a span has no load of a
+      // single float (nor one under a condition, for which the compiler would wait with the loads of V in flight)
+      int blk0 = 0;
+      float ksl = 0.f, vsl = 0.f;
+      auto scale_at = [&](float v, int key) {
+        return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), (key >> c.lgT) - blk0));
+      };
+      // uniform base of a 16-key tile plus 32-bit offsets of the lane that stay the same; where the codes end with the
+      // step's first tile (T = 16), the second one re-reads it and is masked
+      const int64_t head = (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
+      const int ss = (int)c.c_ss;
+      const unsigned ko = (unsigned)(r16 * ss + (D >= 64 ? 16 : 8) * g);
+      unsigned vo[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vo[j] = (unsigned)((4 * g + j) * ss + r16 * NE);
-    auto tile = [&](int k0, int a) { return head + (int64_t)(k0 + (a && k0 + 16 < end ? 16 : 0)) * c.c_ss; };
-    typename Raw<D>::K k[2][NH];
-    auto load_k = [&](int k0) {
+      for (int j = 0; j < 4; ++j) vo[j] = (unsigned)((4 * g + j) * ss + r16 * NE);
+      auto tile = [&](int k0, int a) { return head + (int64_t)(k0 + (a && k0 + 16 < end ? 16 : 0)) * c.c_ss; };
+      typename Raw<D>::K k[2][NH];
+      auto load_k = [&](int k0) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const uint8_t* base = (const uint8_t*)c.kc + tile(k0, a);
+        for (int a = 0; a < 2; ++a) {
+          const uint8_t* base = (const uint8_t*)c.kc + tile(k0, a);
 #pragma unroll
-        for (int x = 0; x < NH; ++x) k[a][x] = *reinterpret_cast<const typename Raw<D>::K*>(base + ko + 64 * x);
+          for (int x = 0; x < NH; ++x) k[a][x] = *reinterpret_cast<const typename Raw<D>::K*>(base + ko + 64 * x);
+        }
+      };
+      load_k(first);
+      for (int span = first; span < end; span += 64 << c.lgT) {
+        blk0 = span >> c.lgT;
+        if (blk0 + lane < end >> c.lgT) {
+          const int64_t off = (int64_t)b * c.s_sb + (int64_t)h * c.s_sh + (int64_t)(blk0 + lane) * c.s_sn;
+          ksl = c.ks[off];
+          vsl = c.vs[off];
+        }
+        const int span_end = min(end, span + (64 << c.lgT) - 127);
+        for (int k0 = span; k0 < span_end; k0 += 128) {
+          typename Raw<D>::V v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            v[j] = *reinterpret_cast<const typename Raw<D>::V*>((const uint8_t*)c.vc + tile(k0, j >> 2) + vo[j & 3]);
+          f32x4 s[2];
+          float vs[2];
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+              bf16x8 kb;
+              if constexpr (D >= 64) {
+                widen4<E4M3>(k[a][i >> 1][2 * (i & 1)], kb, 0);
+                widen4<E4M3>(k[a][i >> 1][2 * (i & 1) + 1], kb, 4);
+              } else {
+                widen4<E4M3>(k[a][0].x, kb, 0);
+                widen4<E4M3>(k[a][0].y, kb, 4);
+              }
+              s[a] = mfma16(kb, qf[i], s[a]);
+            }
+            const int key = a && k0 + 16 < end ? k0 + 16 : k0;
+            const float f = sl2 * scale_at(ksl, key);
+            vs[a] = scale_at(vsl, key);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[a][r] *= f;
+          }
+          if (k0 + 16 >= end) s[1] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          load_k(k0 + 128 < end ? k0 + 128 : k0);   // the last turn re-reads its own keys: no branch around loads
+          st.step(s, vs, [&](int e) { return column<E4M3>(v, e); });
+        }
       }
-    };
-    load_k(first);
-    for (int k0 = first; k0 < end; k0 += 128) {
-      typename Raw<D>::V v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = *reinterpret_cast<const typename Raw<D>::V*>((const uint8_t*)c.vc + tile(k0, j >> 2) + vo[j & 3]);
+    }
+    // the open block's bf16 rows lie in the row's last turn (T divides 128): 32 of them a wave
+    const int u0 = 32 * wave, rows = t1 == nt ? n - full : 0;
+    if (u0 < rows) {
+      const bf16* kt = (const bf16*)c.kt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
+      const bf16* vt = (const bf16*)c.vt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
       f32x4 s[2];
-      float vs[2];
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const bf16* src = kt + (int64_t)min(u0 + 16 * a + r16, rows - 1) * c.t_ss;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          bf16x8 kb;
-          if constexpr (D >= 64) {
-            widen4<E4M3>(k[a][i >> 1][2 * (i & 1)], kb, 0);
-            widen4<E4M3>(k[a][i >> 1][2 * (i & 1) + 1], kb, 4);
-          } else {
-            widen4<E4M3>(k[a][0].x, kb, 0);
-            widen4<E4M3>(k[a][0].y, kb, 4);
-          }
-          s[a] = mfma16(kb, qf[i], s[a]);
-        }
-        const int key = a && k0 + 16 < end ? k0 + 16 : k0;
-        const float f = sl2 * scale_at(ksl, key);
-        vs[a] = scale_at(vsl, key);
+        for (int i = 0; i < NI; ++i) s[a] = mfma16(*reinterpret_cast<const bf16x8*>(src + dof(i)), qf[i], s[a]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[a][r] *= f;
+        for (int r = 0; r < 4; ++r) s[a][r] = u0 + 16 * a + 4 * g + r < rows ? s[a][r] * sl2 : -INFINITY;
       }
-      if (k0 + 16 >= end) s[1] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      load_k(k0 + 128 < end ? k0 + 128 : k0);   // the last turn re-reads its own keys: no branch around loads
-      st.step(s, vs, [&](int e) { return column<E4M3>(v, e); });
+      typedef __bf16 vrow __attribute__((ext_vector_type(NE)));
+      vrow v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = *reinterpret_cast<const vrow*>(vt + (int64_t)min(u0 + 16 * (j >> 2) + 4 * g + (j & 3), rows - 1) * c.t_ss +
+                                              r16 * NE);
+      const float one[2] = {1.f, 1.f};
+      st.step(s, one, [&](int e) {
+        bf16x8 o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = v[j][e];
+        return o;
+      });
     }
-  }
-  // the open block's bf16 rows, 32 of them a wave
-  const int t0 = 32 * wave, rows = hi - full;
-  if (t0 < rows) {
-    const bf16* kt = (const bf16*)c.kt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
-    const bf16* vt = (const bf16*)c.vt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
-    f32x4 s[2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const bf16* row = kt + (int64_t)min(t0 + 16 * a + r16, rows - 1) * c.t_ss;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) s[a] = mfma16(*reinterpret_cast<const bf16x8*>(row + dof(i)), qf[i], s[a]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[a][r] = t0 + 16 * a + 4 * g + r < rows ? s[a][r] * sl2 : -INFINITY;
-    }
-    typedef __bf16 vrow __attribute__((ext_vector_type(NE)));
-    vrow v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = *reinterpret_cast<const vrow*>(vt + (int64_t)min(t0 + 16 * (j >> 2) + 4 * g + (j & 3), rows - 1) * c.t_ss +
-                                            r16 * NE);
-    const float one[2] = {1.f, 1.f};
-    st.step(s, one, [&](int e) {
-      bf16x8 o;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = v[j][e];
-      return o;
-    });
-  }
 
-  // merge the four waves
-  float l = st.l;
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  if (r16 < nq) {
-    if (g == 0) {
-      sml[wave][r16][0] = st.m;
-      sml[wave][r16][1] = l;
+    // merge the four waves
+    float l = st.l;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (r16 < nq) {
+      if (g == 0) {
+        sml[wave][r16][0] = st.m;
+        sml[wave][r16][1] = l;
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) so[wave][r16][NE * (4 * g + r) + e] = st.acc[e][r];
     }
-#pragma unroll
-    for (int e = 0; e < NE; ++e)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) so[wave][r16][NE * (4 * g + r) + e] = st.acc[e][r];
-  }
-  __syncthreads();
-  for (int i = tid; i < nq * D; i += 256) {
-    const int q = i / D, d = i % D;
-    float M = -INFINITY, L = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sml[w][q][0]);
-    const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float a = fast_exp2(sml[w][q][0] - base);
-      L = fmaf(a, sml[w][q][1], L);
-      o = fmaf(a, so[w][q][d], o);
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == nt;
+    const int64_t slot = 2 * (int64_t)w + (t0 == 0 ? 1 : 0);   // one share that goes on from the last workgroup's row, one
+                                                               // that the next one goes on with
+    if (p.opart && t0 == 0 && tid == 0) {   // who has the row, for kv8_combine_k
+      int* info = p.info + 2 * ((int64_t)b * heads + row);
+      info[0] = w;
+      info[1] = owner_of(line, at + nt - 1) - w + 1;
     }
-    const int64_t row = (int64_t)b * p.Hq + hq0 + q;
-    if (p.units == 1) {
-      ((bf16*)p.out)[row * D + d] = (bf16)(o / L);
-    } else {
-      const int64_t slot = row * p.units + u;
-      p.opart[slot * D + d] = o;
-      if (d == 0) {
-        p.mlpart[2 * slot] = M;
-        p.mlpart[2 * slot + 1] = L;
+    for (int i = tid; i < nq * D; i += 256) {
+      const int q = i / D, d = i % D;
+      float M = -INFINITY, L = 0.f, o = 0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) M = fmaxf(M, sml[x][q][0]);
+      const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float a = fast_exp2(sml[x][q][0] - base);
+        L = fmaf(a, sml[x][q][1], L);
+        o = fmaf(a, so[x][q][d], o);
+      }
+      if (whole) {   // a sequence without keys has a zero output
+        ((bf16*)p.out)[((int64_t)b * p.Hq + hq0 + q) * D + d] = (bf16)(n > 0 ? o / L : 0.f);
+      } else {
+        p.opart[(slot * 16 + q) * D + d] = o;
+        if (d == 0) {
+          p.mlpart[(slot * 16 + q) * 2] = M;
+          p.mlpart[(slot * 16 + q) * 2 + 1] = L;
+        }
       }
     }
+    at += t1 - t0;
+    if (at >= stop) break;
+    t0 = 0;
+    if (++row == heads) {
+      row = 0;
+      n = uni(length_of(p, ++b));
+      nt = turns_of(p, n);
+    }
+    __syncthreads();   // before the next row's sums overwrite these
   }
 }
 
-// One workgroup per (sequence, query head): its waves take the units in turns, then merge.  D / 64 (at least 1) elements a
-// lane.
+// One workgroup per (sequence, query head) joins the shares of a row that several workgroups had: its waves take them in
+// turns, then merge.  D / 64 (at least 1) elements a lane.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_combine_k(KV8DecodeParams p) {
   constexpr int E = D >= 64 ? D / 64 : 1;
-  __shared__ float so[4][D], sl[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;
-  const int n = max(0, min(p.pos[row / p.Hq], p.c.Smax - 1) + 1), nu = min((int)cdiv(n, p.chunk), p.units);
-  if (nu == 0) return;   // zeros already stored
-  const float* ml = p.mlpart + row * p.units * 2;
-  const float* op = p.opart + row * p.units * D;
-  float M = -INFINITY;
-  for (int i = lane; i < nu; i += 64) M = fmaxf(M, ml[2 * i]);
-  M = wave_max(M);
-  const float base = M == -INFINITY ? 0.f : M;
+  __shared__ float so[4][D];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
+  const int hq = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq, G = p.Hq / p.c.Hkv, q = hq % G % 16;
+  const int* info = p.info + 2 * ((int64_t)b * p.c.Hkv * p.tiles + hq / G * p.tiles + hq % G / 16);
+  const int w0 = uni(info[0]), shares = uni(info[1]);
+  if (shares == 1) return;   // stored whole
+  auto slot = [&](int i) { return (2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * 16 + q; };
   const bool active = lane * E < D;
-  float L = 0.f, o[E] = {};
-#pragma unroll 4
-  for (int i = wave; i < nu; i += 4) {
-    const float a = fast_exp2(ml[2 * i] - base);
-    L = fmaf(a, ml[2 * i + 1], L);
-    if (active) {
+  // 64 shares at a time: lane i weighs share i, the wave's own ones among them are added up
+  float M = -INFINITY, L = 0.f, o[E] = {};
+  for (int base = 0; base < shares; base += 64) {
+    float m = -INFINITY, l = 0.f;
+    if (base + lane < shares) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.mlpart + 2 * slot(base + lane));
+      m = ml.x;
+      l = ml.y;
+    }
+    const float mx = fmaxf(M, wave_max(m)), ref = mx == -INFINITY ? 0.f : mx, old = fast_exp2(M - ref);
+    const float a = fast_exp2(m - ref);
+    L = L * old + wave_sum(a * l);
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(a, op[(int64_t)i * D + lane * E + e], o[e]);
+    for (int e = 0; e < E; ++e) o[e] *= old;
+    M = mx;
+    const int n = min(64, shares - base);
+    for (int i0 = wave; i0 < n; i0 += 32) {   // eight loads in flight; past the end the last share again, with weight 0
+      float v[8][E], ai[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = min(i0 + 4 * u, n - 1);
+        ai[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(a), i));
+        if (i0 + 4 * u >= n) ai[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u][e] = p.opart[slot(base + i) * D + (active ? lane * E + e : 0)];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(ai[u], v[u][e], o[e]);
     }
   }
-  if (lane == 0) sl[wave] = L;
   if (active) {
 #pragma unroll
     for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
@@ -516,8 +619,8 @@ __global__ __launch_bounds__(256) void kv8_combine_k(KV8DecodeParams p) {
   __syncthreads();
   if ((int)threadIdx.x < D) {
     const int d = threadIdx.x;
-    const float sum = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]), all = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    ((bf16*)p.out)[row * D + d] = (bf16)(sum / all);
+    const float sum = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
+    ((bf16*)p.out)[((int64_t)b * p.Hq + hq) * D + d] = (bf16)(sum / L);
   }
 }
 
@@ -566,23 +669,18 @@ void kv8_append(const KV8AppendParams& p, hipStream_t st) {
 #undef DPH_KV8_APP
 }
 
-// Keys of one unit of work: enough units to fill the card several times over whatever the batch (ragged sequences then
-// even out), no fewer than a step of each wave, and a multiple of every block size, so that no open block crosses units.
-int kv8_decode_chunk(int B, int Hkv, int Hq, int T, int max_len) {
-  const int64_t rows = (int64_t)B * Hkv * cdiv(Hq / Hkv, 16);
-  const int64_t keys = cdiv(rows * max_len, 1024);
-  return (int)std::min<int64_t>(128 * std::max<int64_t>(1, cdiv(keys, 128)), 64 * T);   // a lane holds a block's scales
-}
+// Workgroups of a call: three to a CU (what the registers allow at once), or one for each turn that the longest sequences could have.
+int kv8_decode_workgroups(int64_t turns) { return (int)std::min<int64_t>(turns, 768); }
 
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t st) {
   const KV8& c = p.c;
   if (c.B == 0) return;
-  const dim3 grid((unsigned)((int64_t)p.units * c.B * c.Hkv * cdiv(p.Hq / c.Hkv, 16)));
+  const dim3 grid((unsigned)p.wgs);
 #define DPH_KV8_DEC(D_)                                                                          \
   do {                                                                                           \
     if (c.e4m3) hipLaunchKernelGGL((kv8_decode_k<true, D_>), grid, dim3(256), 0, st, p);         \
     else hipLaunchKernelGGL((kv8_decode_k<false, D_>), grid, dim3(256), 0, st, p);               \
-    if (p.units > 1) hipLaunchKernelGGL(kv8_combine_k<D_>, dim3((unsigned)(c.B * p.Hq)), dim3(256), 0, st, p); \
+    if (p.opart) hipLaunchKernelGGL(kv8_combine_k<D_>, dim3((unsigned)(c.B * p.Hq)), dim3(256), 0, st, p); \
   } while (0)
   if (c.D == 128) DPH_KV8_DEC(128);
   else if (c.D == 64) DPH_KV8_DEC(64);

@@ -601,13 +601,17 @@ Tensor kv8_decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& v
   p.pos = pos.data_ptr<int>();
   p.out = out.data_ptr();
   p.Hq = (int)n_heads; p.scale = (float)scale;
-  p.chunk = dph::kv8_decode_chunk(p.c.B, p.c.Hkv, p.Hq, p.c.T, (int)max_len);
-  p.units = (int)((max_len + p.chunk - 1) / p.chunk);
-  Tensor opart, ml;
-  if (p.units > 1) {
-    opart = at::empty({p.c.B, n_heads, p.units, p.c.D}, qkv.options().dtype(at::kFloat));
-    ml = at::empty({p.c.B, n_heads, p.units, 2}, qkv.options().dtype(at::kFloat));
-    p.opart = opart.data_ptr<float>(); p.mlpart = ml.data_ptr<float>();
+  p.tiles = (int)((n_heads / n_kv_heads + 15) / 16);
+  const int64_t rows = int64_t(p.c.B) * p.c.Hkv * p.tiles, most = (int64_t(p.c.Smax) + 127) / 128;
+  TORCH_CHECK(rows * most < (int64_t(1) << 31) && int64_t(p.c.B) * n_heads < (int64_t(1) << 24),
+              "kv8_decode_attention: cache too large for one launch");
+  p.wgs = dph::kv8_decode_workgroups(rows * ((max_len + 127) / 128));
+  Tensor opart;
+  if (max_len > 128) {
+    const int64_t shares = int64_t(p.wgs) * 32;
+    opart = at::empty({shares * (p.c.D + 2) + 2 * rows}, qkv.options().dtype(at::kFloat));
+    p.opart = opart.data_ptr<float>(); p.mlpart = p.opart + shares * p.c.D;
+    p.info = reinterpret_cast<int*>(p.mlpart + shares * 2);
   }
   dph::kv8_decode_attention(p, cur_stream());
   return out;
