@@ -532,7 +532,7 @@ dph::KV8 check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const T
   TORCH_CHECK(D == 32 || D == 64 || D == 128, "kv8: head_dim must be 32, 64 or 128");
   TORCH_CHECK(T == 16 || T == 32 || T == 64 || T == 128, "kv8: the block must be 16, 32, 64 or 128 tokens");
   TORCH_CHECK(kt.size(0) == B && kt.size(2) == H && kt.size(3) == D && ks.size(0) == B && ks.size(1) == Smax / T &&
-                  ks.size(2) == H && Smax >= 1 && Smax < (int64_t(1) << 31) - 256 && H >= 1,
+                  ks.size(2) == H && Smax >= 1 && Smax < (int64_t(1) << 30) && H >= 1,
               "kv8: scales [B, Smax / T, Hkv] and tails [B, T, Hkv, D] must match k / v [B, Smax, Hkv, D]");
   TORCH_CHECK(strides_ok(kc, 16) && strides_ok(kt, 8),
               "kv8: head dim contiguous, the other strides multiples of 16 bytes");
