@@ -380,7 +380,7 @@ struct KV8 {
   void* kc; void* vc; int64_t c_sb, c_ss, c_sh;      // codes [B, Smax, Hkv, D]
   float* ks; float* vs; int64_t s_sb, s_sn, s_sh;    // scales [B, Smax / T, Hkv]
   void* kt; void* vt; int64_t t_sb, t_ss, t_sh;      // open block, bf16 [B, T, Hkv, D]
-  int B, Smax, Hkv, D, T, lgT;                       // T = 1 << lgT
+  int B, Smax, Hkv, D, T, lgT, lgC;                  // T = 1 << lgT, D / 8 = 1 << lgC
   int e4m3;                                          // codes are OCP e4m3, else int8
 };
 struct KV8AppendParams {

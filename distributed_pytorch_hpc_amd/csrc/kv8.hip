@@ -60,82 +60,102 @@ __device__ __forceinline__ float round32(double v) {
   asm("" : "+v"(f));
   return f;
 }
-__device__ __forceinline__ bf16x8 rotate8(bf16x8 x, const float* cos_t, const float* sin_t) {
-  const f32x4 co = *reinterpret_cast<const f32x4*>(cos_t), si = *reinterpret_cast<const f32x4*>(sin_t);
+struct Angles {   // of a chunk's four pairs
+  f32x4 c, s;
+};
+__device__ __forceinline__ bf16x8 rotate8(bf16x8 x, const Angles& w) {
   bf16x8 o;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const double a = (double)(float)x[2 * j], b = (double)(float)x[2 * j + 1];
-    const double c = (double)co[j], s = (double)si[j];
+    const double c = (double)w.c[j], s = (double)w.s[j];
     o[2 * j] = (bf16)round32(a * c - b * s);
     o[2 * j + 1] = (bf16)round32(a * s + b * c);
   }
   return o;
 }
 
-// One workgroup per (sequence, K or V head, touched block).  The block is gathered into registers (old rows from the
-// tail, new ones from qkv, keys rotated), reduced to its largest magnitude -- as integers: |bf16| compares like its
-// bits, and infinities and NaN compare above every finite value -- and quantised if this append fills it.  The first
-// touched block's workgroup is the only one that reads the tail, so it also stores the rows of the block left open,
-// after those reads: no other workgroup has to be waited for.  The remaining workgroups rotate q.
+// Two kinds of workgroups.  The first: one per (sequence, K or V head, touched block).  The block is gathered into
+// registers (old rows from the tail, new ones from qkv, keys rotated), reduced to its largest magnitude -- as integers:
+// |bf16| compares like its bits, and infinities and NaN compare above every finite value -- and quantised if this append
+// fills it.  The first touched block's workgroup is the only one that reads the tail, so it also stores the rows of the
+// block left open, after those reads: no other workgroup has to be waited for.  The second kind rotates q, one per new
+// token: a thread keeps its angles and goes from head to head with them.
 template <bool E4M3, int NC>
 __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk, int quant_wgs) {
   const KV8& c = p.c;
-  const int CH = c.D / 8, T = c.T, half = c.D / 2;
-  const int tid = threadIdx.x;
+  const int T = c.T, half = c.D / 2, tid = threadIdx.x;
+  auto angles = [&](int t, int ch) {
+    const int64_t o = (int64_t)t * half + ch * 4;
+    return Angles{*reinterpret_cast<const f32x4*>(p.cos + o), *reinterpret_cast<const f32x4*>(p.sin + o)};
+  };
   if ((int)blockIdx.x >= quant_wgs) {
-    const int64_t i = (int64_t)(blockIdx.x - quant_wgs) * 256 + tid;
-    if (i >= (int64_t)c.B * p.S * p.Hq * CH) return;
-    const int ch = (int)(i % CH);
-    int64_t r = i / CH;
-    const int h = (int)(r % p.Hq);
-    r /= p.Hq;
-    const int s = (int)(r % p.S), b = (int)(r / p.S);
-    const int64_t t = (int64_t)p.pos[b] + s;
-    if (p.pos[b] < 0 || t >= c.Smax) return;   // the host checks capacity; the tables end with the cache
-    bf16* x = (bf16*)p.qkv + (int64_t)b * p.qkv_sb + (int64_t)s * p.qkv_ss + (int64_t)h * c.D + ch * 8;
-    *reinterpret_cast<bf16x8*>(x) =
-        rotate8(*reinterpret_cast<const bf16x8*>(x), p.cos + t * half + ch * 4, p.sin + t * half + ch * 4);
+    const int i = blockIdx.x - quant_wgs, b = i / p.S, s = i - b * p.S;
+    const int pos = p.pos[b];
+    if (pos < 0 || (int64_t)pos + s >= c.Smax) return;   // the host checks capacity; the tables end with the cache
+    const Angles w = angles(pos + s, tid & ((1 << c.lgC) - 1));
+    bf16* x = (bf16*)p.qkv + (int64_t)b * p.qkv_sb + (int64_t)s * p.qkv_ss;
+    const int n = p.Hq << c.lgC;   // chunks; 256 is a multiple of a head's
+    for (int e = tid; e < n; e += 4 * 256) {
+      bf16x8 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const bf16x8*>(x + 8 * (e + 256 * u < n ? e + 256 * u : e));
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (e + 256 * u < n) *reinterpret_cast<bf16x8*>(x + 8 * (e + 256 * u)) = rotate8(v[u], w);
+    }
     return;
   }
   __shared__ unsigned red[4];
   const int j = blockIdx.x % nblk;
-  int r0 = blockIdx.x / nblk;
+  const int r0 = blockIdx.x / nblk;
   const int hh = r0 % (2 * c.Hkv), b = r0 / (2 * c.Hkv);
   const bool is_k = hh < c.Hkv;
   const int h = is_k ? hh : hh - c.Hkv;
   const int pos = p.pos[b];
   if (pos < 0 || pos >= c.Smax) return;   // whole workgroup, before any barrier
   const int n = (int)min((int64_t)pos + p.S, (int64_t)c.Smax);
-  const int blk = (pos >> c.lgT) + j, t0 = blk * T;
+  const int blk = (pos >> c.lgT) + j, t0 = blk << c.lgT;
   if (t0 >= n) return;
   const bool full = n - t0 >= T;
   if (!full && j > 0) return;
 
   bf16* src = (bf16*)p.qkv + (int64_t)b * p.qkv_sb + (int64_t)(p.Hq + hh) * c.D;   // row s of this head: + s * qkv_ss
   bf16* tail = (bf16*)(is_k ? c.kt : c.vt) + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
-  auto fresh = [&](int t, int ch) -> bf16x8 {   // new row t; keys are rotated, in qkv too
-    bf16* x = src + (int64_t)(t - pos) * p.qkv_ss + ch * 8;
-    bf16x8 v = *reinterpret_cast<const bf16x8*>(x);
-    if (is_k) {
-      v = rotate8(v, p.cos + (int64_t)t * half + ch * 4, p.sin + (int64_t)t * half + ch * 4);
-      *reinterpret_cast<bf16x8*>(x) = v;
-    }
-    return v;
-  };
+  const int chunks = T << c.lgC, mask = (1 << c.lgC) - 1;
   if (full) {
     bf16x8 val[NC];
+    Angles w[NC];
+    // every load at once: rows come from one of two places by address, threads past a small block take its last chunk
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int e = min(i * 256 + tid, chunks - 1), row = e >> c.lgC, ch = e & mask, t = t0 + row;
+      val[i] = *reinterpret_cast<const bf16x8*>(t < pos ? tail + (int64_t)row * c.t_ss + ch * 8
+                                                        : src + (int64_t)(t - pos) * p.qkv_ss + ch * 8);
+    }
+    if (is_k) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int e = min(i * 256 + tid, chunks - 1);
+        w[i] = angles(t0 + (e >> c.lgC), e & mask);
+      }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int e = min(i * 256 + tid, chunks - 1), t = t0 + (e >> c.lgC);
+        const bf16x8 r = rotate8(val[i], w[i]);
+        if (t >= pos) {
+          val[i] = r;
+          if (i * 256 + tid < chunks)
+            *reinterpret_cast<bf16x8*>(src + (int64_t)(t - pos) * p.qkv_ss + (e & mask) * 8) = r;
+        }
+      }
+    }
     unsigned mx = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int e = i * 256 + tid;
-      if (e < T * CH) {
-        const int row = e / CH, ch = e % CH, t = t0 + row;
-        val[i] = t < pos ? *reinterpret_cast<const bf16x8*>(tail + (int64_t)row * c.t_ss + ch * 8) : fresh(t, ch);
-        const u32x4 w = __builtin_bit_cast(u32x4, val[i]);
+      const u32x4 u = __builtin_bit_cast(u32x4, val[i]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx = max(mx, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-      }
+      for (int k = 0; k < 4; ++k) mx = max(mx, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, o, 64));
@@ -150,15 +170,14 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int e = i * 256 + tid;
-      if (e < T * CH) {
-        const int row = e / CH, ch = e % CH;
+      if (e < chunks) {
         float lo[4], hi[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           lo[k] = finite ? (float)val[i][k] * inv : 0.f;
           hi[k] = finite ? (float)val[i][4 + k] * inv : 0.f;
         }
-        *reinterpret_cast<uint2*>(code + (int64_t)(t0 + row) * c.c_ss + ch * 8) =
+        *reinterpret_cast<uint2*>(code + (int64_t)(t0 + (e >> c.lgC)) * c.c_ss + (e & mask) * 8) =
             make_uint2(pack4<E4M3>(lo), pack4<E4M3>(hi));
       }
     }
@@ -166,31 +185,16 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
   }
   if (j == 0) {   // the barrier above ordered the tail's reads before these writes
     const int o0 = n >> c.lgT << c.lgT, from = max(o0, pos);
-    for (int e = tid; e < (n - from) * CH; e += 256) {
-      const int t = from + e / CH, ch = e % CH;
-      *reinterpret_cast<bf16x8*>(tail + (int64_t)(t - o0) * c.t_ss + ch * 8) = fresh(t, ch);
+    for (int e = tid; e < (n - from) << c.lgC; e += 256) {
+      const int t = from + (e >> c.lgC), ch = e & mask;
+      bf16* x = src + (int64_t)(t - pos) * p.qkv_ss + ch * 8;
+      bf16x8 v = *reinterpret_cast<const bf16x8*>(x);
+      if (is_k) {
+        v = rotate8(v, angles(t, ch));
+        *reinterpret_cast<bf16x8*>(x) = v;
+      }
+      *reinterpret_cast<bf16x8*>(tail + (int64_t)(t - o0) * c.t_ss + ch * 8) = v;
     }
-  }
-}
-
-// 8 elements of row t of the cache that holds n rows, in fp32
-template <bool E4M3>
-__device__ __forceinline__ void row8(const KV8& c, bool is_k, int b, int h, int t, int n, int ch, float (&o)[8]) {
-  if (t < n >> c.lgT << c.lgT) {
-    const uint2 r = *reinterpret_cast<const uint2*>((const uint8_t*)(is_k ? c.kc : c.vc) + (int64_t)b * c.c_sb +
-                                                    (int64_t)t * c.c_ss + (int64_t)h * c.c_sh + ch * 8);
-    const float sc = (is_k ? c.ks : c.vs)[(int64_t)b * c.s_sb + (int64_t)(t >> c.lgT) * c.s_sn + (int64_t)h * c.s_sh];
-    float lo[4], hi[4];
-    unpack4<E4M3>(r.x, lo);
-    unpack4<E4M3>(r.y, hi);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      o[k] = lo[k] * sc;
-      o[4 + k] = hi[k] * sc;
-    }
-  } else {
-    Vec8<bf16>::load((const bf16*)(is_k ? c.kt : c.vt) + (int64_t)b * c.t_sb + (int64_t)(t & (c.T - 1)) * c.t_ss +
-                         (int64_t)h * c.t_sh + ch * 8, o);
   }
 }
 
@@ -624,25 +628,61 @@ __global__ __launch_bounds__(256) void kv8_combine_k(KV8DecodeParams p) {
   }
 }
 
-template <bool E4M3>
-__global__ __launch_bounds__(256) void kv8_read_k(KV8ReadParams p) {
+// Read-back: a workgroup per (sequence, K or V, head, 8192 / D output rows), two chunks of 16 elements a thread.  Bound by
+// its 3 bytes an element; a head's rows are read next to each other, rows of an output are written D elements at a time.
+template <bool E4M3, int D>
+__global__ __launch_bounds__(256) void kv8_read_k(KV8ReadParams p, int nrow) {
+  constexpr int CH = D / 16, R = 8192 / D;
   const KV8& c = p.c;
-  const int CH = c.D / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)c.B * p.count * c.Hkv * 2 * CH) return;
-  const int ch = (int)(i % CH);
-  int64_t r = i / CH;
-  const int h = (int)(r % c.Hkv);
-  r /= c.Hkv;
-  const int s = (int)(r % p.count);
-  r /= p.count;
-  const int b = (int)(r % c.B);
-  const bool is_k = r < c.B;
-  const int n = max(0, min(p.pos[b], c.Smax)), t = n - p.count + s;
-  float v[8] = {};
-  if (t >= 0) row8<E4M3>(c, is_k, b, h, t, n, ch, v);
-  Vec8<bf16>::store((bf16*)(is_k ? p.ko : p.vo) + (int64_t)b * p.o_sb + (int64_t)s * p.o_ss + (int64_t)h * p.o_sh + ch * 8,
-                    v);
+  const int part = blockIdx.x % nrow;
+  int id = blockIdx.x / nrow;
+  const int h = id % c.Hkv;
+  id /= c.Hkv;
+  const bool is_k = id & 1;
+  const int b = id >> 1;
+  const int n = max(0, min(p.pos[b], c.Smax)), full = n >> c.lgT << c.lgT;
+  const uint8_t* code = (const uint8_t*)(is_k ? c.kc : c.vc) + (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
+  const float* scale = (is_k ? c.ks : c.vs) + (int64_t)b * c.s_sb + (int64_t)h * c.s_sh;
+  const bf16* tail = (const bf16*)(is_k ? c.kt : c.vt) + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
+  bf16* out = (bf16*)(is_k ? p.ko : p.vo) + (int64_t)b * p.o_sb + (int64_t)h * p.o_sh;
+  const int ch = threadIdx.x % CH;
+  int s[2], t[2];
+  u32x4 raw[2] = {};
+  float sc[2] = {};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    s[i] = part * R + i * (R / 2) + (int)threadIdx.x / CH;
+    t[i] = n - p.count + s[i];
+  }
+  if (full > 0) {   // whole workgroup: rows that are not codes read the nearest ones
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = max(0, min(t[i], full - 1));
+      raw[i] = *reinterpret_cast<const u32x4*>(code + (int64_t)r * c.c_ss + ch * 16);
+      sc[i] = scale[(int64_t)(r >> c.lgT) * c.s_sn];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (s[i] >= p.count) continue;
+    bf16x8 o[2] = {};
+    if (t[i] >= full) {
+      const bf16* src = tail + (int64_t)(t[i] - full) * c.t_ss + ch * 16;
+      o[0] = *reinterpret_cast<const bf16x8*>(src);
+      o[1] = *reinterpret_cast<const bf16x8*>(src + 8);
+    } else if (t[i] >= 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float f[4];
+        unpack4<E4M3>(raw[i][k], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k >> 1][4 * (k & 1) + e] = (bf16)(f[e] * sc[i]);
+      }
+    }
+    bf16* dst = out + (int64_t)s[i] * p.o_ss + ch * 16;
+    *reinterpret_cast<bf16x8*>(dst) = o[0];
+    *reinterpret_cast<bf16x8*>(dst + 8) = o[1];
+  }
 }
 
 }  // namespace
@@ -650,17 +690,16 @@ __global__ __launch_bounds__(256) void kv8_read_k(KV8ReadParams p) {
 void kv8_append(const KV8AppendParams& p, hipStream_t st) {
   const KV8& c = p.c;
   if (c.B == 0 || p.S == 0) return;
-  const int CH = c.D / 8;
   const int nblk = (p.S + c.T - 2) / c.T + 1;   // blocks that S rows can touch, whatever their first position
   const int quant = c.B * 2 * c.Hkv * nblk;
-  const dim3 grid((unsigned)(quant + cdiv((int64_t)c.B * p.S * p.Hq * CH, 256)));
+  const dim3 grid((unsigned)(quant + c.B * p.S));
 #define DPH_KV8_APP(E_, NC_) hipLaunchKernelGGL((kv8_append_k<E_, NC_>), grid, dim3(256), 0, st, p, nblk, quant)
 #define DPH_KV8_APP_E(NC_)               \
   do {                                   \
     if (c.e4m3) DPH_KV8_APP(true, NC_);  \
     else DPH_KV8_APP(false, NC_);        \
   } while (0)
-  const int chunks = c.T * CH;   // 16-B chunks of one block, in registers: at most 8 a thread
+  const int chunks = c.T << c.lgC;   // 16-B chunks of one block, in registers: at most 8 a thread
   if (chunks <= 256) DPH_KV8_APP_E(1);
   else if (chunks <= 512) DPH_KV8_APP_E(2);
   else if (chunks <= 1024) DPH_KV8_APP_E(4);
@@ -689,11 +728,19 @@ void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t st) {
 }
 
 void kv8_read(const KV8ReadParams& p, hipStream_t st) {
-  const int64_t total = (int64_t)p.c.B * p.count * p.c.Hkv * 2 * (p.c.D / 8);
-  if (total == 0) return;
-  const dim3 grid((unsigned)cdiv(total, 256));
-  if (p.c.e4m3) hipLaunchKernelGGL(kv8_read_k<true>, grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(kv8_read_k<false>, grid, dim3(256), 0, st, p);
+  const KV8& c = p.c;
+  if (c.B == 0 || p.count == 0) return;
+  const int nrow = (int)cdiv((int64_t)p.count * c.D, 8192);
+  const dim3 grid((unsigned)((int64_t)nrow * c.Hkv * 2 * c.B));
+#define DPH_KV8_READ(D_)                                                                              \
+  do {                                                                                                \
+    if (c.e4m3) hipLaunchKernelGGL((kv8_read_k<true, D_>), grid, dim3(256), 0, st, p, nrow);          \
+    else hipLaunchKernelGGL((kv8_read_k<false, D_>), grid, dim3(256), 0, st, p, nrow);                \
+  } while (0)
+  if (c.D == 128) DPH_KV8_READ(128);
+  else if (c.D == 64) DPH_KV8_READ(64);
+  else DPH_KV8_READ(32);
+#undef DPH_KV8_READ
 }
 
 }  // namespace dph

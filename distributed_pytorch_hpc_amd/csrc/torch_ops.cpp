@@ -543,7 +543,8 @@ dph::KV8 check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const T
   c.ks = ks.data_ptr<float>(); c.vs = vs.data_ptr<float>();
   c.s_sb = ks.stride(0); c.s_sn = ks.stride(1); c.s_sh = ks.stride(2);
   c.kt = kt.data_ptr(); c.vt = vt.data_ptr(); c.t_sb = kt.stride(0); c.t_ss = kt.stride(1); c.t_sh = kt.stride(2);
-  c.B = (int)B; c.Smax = (int)Smax; c.Hkv = (int)H; c.D = (int)D; c.T = (int)T; c.lgT = __builtin_ctz((unsigned)T); c.e4m3 = e4m3 ? 1 : 0;
+  c.B = (int)B; c.Smax = (int)Smax; c.Hkv = (int)H; c.D = (int)D; c.T = (int)T; c.lgT = __builtin_ctz((unsigned)T);
+  c.lgC = __builtin_ctz((unsigned)(D / 8)); c.e4m3 = e4m3 ? 1 : 0;
   return c;
 }
 
@@ -579,7 +580,8 @@ void kv8_append_(Tensor& qkv, Tensor& kc, Tensor& vc, Tensor& ks, Tensor& vs, Te
   no_overlap({&qkv, &kc, &vc, &ks, &vs, &kt, &vt});
   const int64_t S = qkv.size(1);
   TORCH_CHECK(S <= p.c.Smax, "kv8_append: ", S, " new tokens for a cache of ", p.c.Smax);
-  TORCH_CHECK(qkv.numel() / 8 < (int64_t(1) << 32) - (int64_t(1) << 24), "kv8_append: qkv too large for one launch");
+  TORCH_CHECK(int64_t(p.c.B) * S < (int64_t(1) << 23) && int64_t(p.c.B) * p.c.Hkv * 2 * (S / p.c.T + 2) < (int64_t(1) << 23),
+              "kv8_append: qkv too large for one launch");
   p.qkv = qkv.data_ptr(); p.qkv_sb = qkv.stride(0); p.qkv_ss = qkv.stride(1);
   p.pos = pos.data_ptr<int>(); p.cos = cos.data_ptr<float>(); p.sin = sin.data_ptr<float>();
   p.S = (int)S; p.Hq = (int)n_heads;
@@ -631,7 +633,8 @@ void kv8_read_(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tenso
   TORCH_CHECK(strides_ok(ko, 8), "kv8_read: outputs need a contiguous head dim and strides that are multiples of 8");
   check_align16(ko, "k_out"); check_align16(vo, "v_out");
   no_overlap({&ko, &vo});
-  TORCH_CHECK(2 * ko.numel() / 8 < (int64_t(1) << 32) - 256, "kv8_read: too large for one launch");
+  TORCH_CHECK(int64_t(p.c.B) * p.c.Hkv * 2 * (ko.size(1) * p.c.D / 8192 + 1) < (int64_t(1) << 24),
+              "kv8_read: too large for one launch");
   p.pos = pos.data_ptr<int>();
   p.ko = ko.data_ptr(); p.vo = vo.data_ptr(); p.o_sb = ko.stride(0); p.o_ss = ko.stride(1); p.o_sh = ko.stride(2);
   p.count = (int)ko.size(1);
