@@ -91,15 +91,20 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
   };
   if ((int)blockIdx.x >= quant_wgs) {
     const int i = blockIdx.x - quant_wgs, b = i / p.S, s = i - b * p.S;
-    const int pos = p.pos[b];
-    if (pos < 0 || (int64_t)pos + s >= c.Smax) return;   // the host checks capacity; the tables end with the cache
-    const Angles w = angles(pos + s, tid & ((1 << c.lgC) - 1));
     bf16* x = (bf16*)p.qkv + (int64_t)b * p.qkv_sb + (int64_t)s * p.qkv_ss;
     const int n = p.Hq << c.lgC;   // chunks; 256 is a multiple of a head's
-    for (int e = tid; e < n; e += 4 * 256) {
-      bf16x8 v[4];
+    bf16x8 v[4];
+    auto load = [&](int e) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const bf16x8*>(x + 8 * (e + 256 * u < n ? e + 256 * u : e));
+    };
+    if (tid >= n) return;
+    load(tid);   // before the position is known: only the angles wait for it
+    const int64_t t = (int64_t)p.pos[b] + s;
+    if (t < s || t >= c.Smax) return;   // the host checks capacity; the tables end with the cache
+    const Angles w = angles((int)t, tid & ((1 << c.lgC) - 1));
+    for (int e = tid; e < n; e += 4 * 256) {
+      if (e != tid) load(e);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (e + 256 * u < n) *reinterpret_cast<bf16x8*>(x + 8 * (e + 256 * u)) = rotate8(v[u], w);
@@ -107,8 +112,7 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
     return;
   }
   __shared__ unsigned red[4];
-  const int j = blockIdx.x % nblk;
-  const int r0 = blockIdx.x / nblk;
+  const int j = blockIdx.x % nblk, r0 = blockIdx.x / nblk;
   const int hh = r0 % (2 * c.Hkv), b = r0 / (2 * c.Hkv);
   const bool is_k = hh < c.Hkv;
   const int h = is_k ? hh : hh - c.Hkv;

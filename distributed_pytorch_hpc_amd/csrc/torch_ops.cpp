@@ -641,6 +641,16 @@ void kv8_read_(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tenso
   dph::kv8_read(p, cur_stream());
 }
 
+std::tuple<Tensor, Tensor> kv8_read(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+                                    const Tensor& kt, const Tensor& vt, const Tensor& pos, int64_t count) {
+  TORCH_CHECK(kc.dim() == 4 && count >= 0 && count <= kc.size(1), "kv8_read: count ", count, " is not in 0 .. Smax");
+  c10::DeviceGuard g(kc.device());
+  auto ko = at::empty({kc.size(0), count, kc.size(2), kc.size(3)}, kc.options().dtype(at::kBFloat16));
+  auto vo = at::empty(ko.sizes(), ko.options());
+  kv8_read_(kc, vc, ks, vs, kt, vt, pos, ko, vo);
+  return {ko, vo};
+}
+
 Tensor process_logits(const Tensor& logits, const c10::optional<Tensor>& tokens, const c10::optional<Tensor>& lengths,
                       const c10::optional<Tensor>& prompt_lengths, const c10::optional<Tensor>& repetition,
                       const c10::optional<Tensor>& presence, const c10::optional<Tensor>& frequency,
@@ -1939,6 +1949,8 @@ TORCH_LIBRARY(dph, m) {
         "Tensor v_tail, Tensor pos, int n_heads, int n_kv_heads, float scale, int max_len) -> Tensor");
   m.def("kv8_read_(Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor k_tail, Tensor v_tail, Tensor pos, "
         "Tensor(a!) k_out, Tensor(b!) v_out) -> ()");
+  m.def("kv8_read(Tensor k, Tensor v, Tensor k_scale, Tensor v_scale, Tensor k_tail, Tensor v_tail, Tensor pos, "
+        "int count) -> (Tensor, Tensor)");
   m.def("process_logits(Tensor logits, Tensor? tokens=None, Tensor? lengths=None, Tensor? prompt_lengths=None, "
         "Tensor? repetition=None, Tensor? presence=None, Tensor? frequency=None, Tensor? bias=None, "
         "Tensor? mask=None) -> Tensor");
@@ -2036,6 +2048,7 @@ TORCH_LIBRARY_IMPL(dph, CUDA, m) {
   m.impl("kv8_append_", &kv8_append_);
   m.impl("kv8_decode_attention", &kv8_decode_attention);
   m.impl("kv8_read_", &kv8_read_);
+  m.impl("kv8_read", &kv8_read);
   m.impl("process_logits", &process_logits);
   m.impl("decode_attention", &decode_attention);
   m.impl("skinny_linear", &skinny_linear);

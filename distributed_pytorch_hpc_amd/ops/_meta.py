@@ -329,6 +329,12 @@ def _kv8_read(k, v, k_scale, v_scale, k_tail, v_tail, pos, k_out, v_out):
     return None
 
 
+@register_fake("dph::kv8_read")
+def _kv8_read_new(k, v, k_scale, v_scale, k_tail, v_tail, pos, count):
+    o = k_tail.new_empty((k.shape[0], count, k.shape[2], k.shape[3]))
+    return o, torch.empty_like(o)
+
+
 @register_fake("dph::process_logits")
 def _process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repetition=None, presence=None,
                     frequency=None, bias=None, mask=None):

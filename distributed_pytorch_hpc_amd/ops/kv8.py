@@ -206,17 +206,21 @@ def kv8_read(cache: KV8Cache, pos: torch.Tensor, count: int,
              out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The last ``count`` of every sequence's pos[b] stored rows as bf16 (k, v) [B, count, Hkv, D]; rows before the first
     token are zero.  ``out``: two tensors (views) of that shape to write into."""
-    bsz, smax, h, d = cache.k.shape
-    if not 0 <= count <= smax:
-        raise ValueError(f"kv8_read: count {count} is not in 0 .. {smax}")
-    if out is None:
-        out = tuple(torch.empty(bsz, count, h, d, dtype=torch.bfloat16, device=cache.k.device) for _ in range(2))
-    elif any(tuple(o.shape) != (bsz, count, h, d) for o in out):
-        raise ValueError(f"kv8_read: out must be two tensors of shape {(bsz, count, h, d)}")
     if _lib.use_native(cache.k):
+        if out is None:
+            return _lib.ops().kv8_read(*cache, pos, count)
+        if any(o.dim() != 4 or o.shape[1] != count for o in out):
+            raise ValueError(f"kv8_read: out must be two [B, {count}, Hkv, D] tensors")
         _lib.ops().kv8_read_(*cache, pos, *out)
-    else:
-        _check(cache, pos)
-        for o, x in zip(out, kv8_read_reference(cache, pos, count)):
-            o.copy_(x)
+        return out
+    _check(cache, pos)
+    if not 0 <= count <= cache.k.shape[1]:
+        raise ValueError(f"kv8_read: count {count} is not in 0 .. {cache.k.shape[1]}")
+    kv = kv8_read_reference(cache, pos, count)
+    if out is None:
+        return kv
+    if any(o.shape != x.shape for o, x in zip(out, kv)):
+        raise ValueError(f"kv8_read: out must be two tensors of shape {tuple(kv[0].shape)}")
+    for o, x in zip(out, kv):
+        o.copy_(x)
     return out
