@@ -36,8 +36,10 @@ def main():
     ap.add_argument("--prompt", type=int, default=1024)
     ap.add_argument("--steps", type=int, default=64)
     ap.add_argument("--modes", nargs="+", choices=["eager", "graph"], default=["eager", "graph"])
-    ap.add_argument("--kv-dtype", choices=["bf16", "fp8"], default="bf16",
-                    help="KV-cache entries: bf16, or OCP e4m3 (half the cache bytes; opt-in, lossy)")
+    ap.add_argument("--kv-dtype", choices=["bf16", "fp8", "int8"], default="bf16",
+                    help="KV-cache entries: bf16, OCP e4m3 or int8 (half the cache bytes; opt-in, lossy)")
+    ap.add_argument("--kv-block", type=int, default=None,
+                    help="tokens that share a scale (fp8: without it one scale for the cache; int8: 64)")
     ap.add_argument("--json", default=None)
     args = ap.parse_args()
 
@@ -50,7 +52,8 @@ def main():
     margs = get_preset(args.model, max_seq_len=max(margs.max_seq_len, args.prompt + args.steps + 16))
     model = build_llama(margs, device="cuda", dtype=torch.bfloat16, seed=0)
     wbytes = sum(p.numel() * p.element_size() for p in model.parameters()) - margs.vocab_size * margs.dim * 2
-    kv_dtype = torch.float8_e4m3fn if args.kv_dtype == "fp8" else None
+    kv_dtype = {"bf16": None, "fp8": torch.float8_e4m3fn, "int8": torch.int8}[args.kv_dtype]
+    kv_block = args.kv_block or (64 if kv_dtype == torch.int8 else None)
     kv_per_tok = margs.n_layers * 2 * margs.kv_heads * margs.head_dim * (1 if kv_dtype is not None else 2)
     rows = []
     for B in args.batches:
@@ -58,7 +61,7 @@ def main():
         prompts = torch.randint(0, margs.vocab_size, (B, args.prompt), device="cuda")
         rec = {"batch": B, "prompt": args.prompt, "decode_steps": args.steps}
         for graphs in [m == "graph" for m in args.modes]:
-            gen = Generator(model, B, max_len, graphs=graphs, dtype=kv_dtype)
+            gen = Generator(model, B, max_len, graphs=graphs, dtype=kv_dtype, kv_block=kv_block)
             gen.prefill(prompts)   # warm-up (library heuristics, allocator)
             gen.reset()
             torch.cuda.synchronize()
@@ -88,7 +91,8 @@ def main():
             torch.cuda.empty_cache()
         rows.append(rec)
         print(json.dumps(rec), flush=True)
-    res = {"model": args.model, "dtype": "bf16", "kv_cache": args.kv_dtype, "data": "synthetic prompts, random-init weights",
+    res = {"model": args.model, "dtype": "bf16", "kv_cache": args.kv_dtype, "kv_block": kv_block,
+           "data": "synthetic prompts, random-init weights",
            "weight_bytes": wbytes, "kv_bytes_per_token": kv_per_tok, "rows": rows}
     if args.json:
         with open(args.json, "w") as fh:

@@ -11,7 +11,8 @@ The reference trains only (its llama2_model.py has no KV cache); this is the ser
   batch -- ~10 kernels per layer.  The first decode step runs eagerly (lazy library set-up, allocator warm-up), the
   second captures the step into a HIP graph, every later one is a single replay: the kernels read the token buffer
   and the per-sequence positions from device memory, so nothing in the step depends on the host.
-* sampling (greedy, temperature, top-k) runs on the logits outside the graph.
+* sampling (greedy, temperature, top-k) runs on the logits outside the graph, after the penalties, biases and grammar
+  masks of ``controls`` (controls.py, one kernel a step).
 """
 from __future__ import annotations
 
@@ -21,14 +22,16 @@ from typing import Optional, Sequence
 import torch
 
 from ..models.llama2 import KVCache, Transformer
+from .controls import LogitControls, LogitProcessor
 
 
 class Generator:
     def __init__(self, model: Transformer, batch: int, max_len: int, graphs: Optional[bool] = None,
-                 dtype: torch.dtype | None = None, kv_scale: float = 1.0):
-        """``dtype``: KV-cache element type (default the model's; ``torch.float8_e4m3fn`` halves the cache bytes)."""
+                 dtype: torch.dtype | None = None, kv_scale: float = 1.0, kv_block: Optional[int] = None):
+        """``dtype``: KV-cache element type (default the model's; ``torch.float8_e4m3fn`` halves the cache bytes, and so
+        does ``torch.int8`` or e4m3 with ``kv_block=64``, a scale for every 64 tokens of a KV head)."""
         self.model = model
-        self.cache = KVCache(model, batch, max_len, dtype=dtype, kv_scale=kv_scale)
+        self.cache = KVCache(model, batch, max_len, dtype=dtype, kv_scale=kv_scale, kv_block=kv_block)
         dev = self.cache.pos.device
         self.device = dev
         if graphs is None:
@@ -115,26 +118,57 @@ class Generator:
             x = x.masked_fill(x < kth, float("-inf"))
         return torch.multinomial(torch.softmax(x, -1), 1, generator=generator).view(-1)
 
+    def processor(self, prompts: Sequence[Sequence[int]],
+                  controls: LogitControls | Sequence[Optional[LogitControls]] | None) -> Optional[LogitProcessor]:
+        """The processor of a batch of prompts, or None without controls."""
+        if controls is None or isinstance(controls, LogitControls):
+            controls = [controls] * len(prompts)
+        if len(controls) != len(prompts):
+            raise ValueError(f"{len(controls)} controls for {len(prompts)} prompts")
+        if all(c is None for c in controls):
+            return None
+        proc = LogitProcessor(len(prompts), self.cache.max_len + 1, self.model.vocab_size, self.device)
+        for i, (p, c) in enumerate(zip(prompts, controls)):
+            if c is not None:
+                proc.start(i, p, c)
+        return proc
+
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]] | torch.Tensor, max_new_tokens: int,
                  temperature: float = 0.0, top_k: Optional[int] = None, eos_id: Optional[int] = None,
-                 generator: Optional[torch.Generator] = None) -> list:
-        """Prompts (B lists of ids or LongTensor [B, S]) -> B lists of ids: prompt + up to ``max_new_tokens``."""
+                 generator: Optional[torch.Generator] = None,
+                 controls: LogitControls | Sequence[Optional[LogitControls]] | None = None) -> list:
+        """Prompts (B lists of ids or LongTensor [B, S]) -> B lists of ids: prompt + up to ``max_new_tokens``.
+        ``controls``: one ``LogitControls`` for every sequence, or one (or None) each."""
         rows = prompts.tolist() if isinstance(prompts, torch.Tensor) else [list(p) for p in prompts]
         longest = max(len(p) for p in rows)
         if longest + max_new_tokens > self.cache.max_len + 1:
             raise ValueError(f"prompt {longest} + {max_new_tokens} new tokens exceed the cache ({self.cache.max_len})")
+        proc = self.processor(rows, controls)
+        starts = [len(p) for p in rows]
+        if proc is not None:
+            for i in range(len(rows)):
+                proc.restrict(i, [])
         self.reset()
         logits = self.prefill(prompts if isinstance(prompts, torch.Tensor) else rows)
         done = [False] * len(rows)
         for step in range(max_new_tokens):
+            if proc is not None:
+                logits = proc(logits)
             tok = self.sample(logits, temperature, top_k, generator)
+            if proc is not None:
+                proc.push(tok)
             for i, t in enumerate(tok.tolist()):
                 if not done[i]:
                     rows[i].append(t)
                     done[i] = eos_id is not None and t == eos_id
+                    if done[i] and proc is not None:
+                        proc.stop(i)
             if all(done) or step == max_new_tokens - 1:
                 break
+            if proc is not None:
+                for i, r in enumerate(rows):
+                    proc.restrict(i, r[starts[i]:])
             logits = self.decode(tok)
         return rows
 
@@ -146,6 +180,7 @@ class Request:
     eos_id: Optional[int] = None
     output: list = field(default_factory=list)   # generated ids
     done: bool = False
+    controls: Optional[LogitControls] = None
 
     def _push(self, tok: int) -> None:
         self.output.append(tok)
@@ -173,15 +208,20 @@ class ContinuousBatcher:
         self.slots: list = [None] * generator.batch
         self.queue: list = []
         self._next = torch.zeros(generator.batch, dtype=torch.long, device=generator.device)
+        self._proc: Optional[LogitProcessor] = None   # with the first request that has controls
+        self._finished: list = []                     # not yet returned (kept when a step raises)
         generator.reset()
 
-    def submit(self, prompt: Sequence[int], max_new_tokens: int, eos_id: Optional[int] = None) -> Request:
+    def submit(self, prompt: Sequence[int], max_new_tokens: int, eos_id: Optional[int] = None,
+               controls: Optional[LogitControls] = None) -> Request:
         if not prompt or max_new_tokens < 1:
             raise ValueError("ContinuousBatcher: empty prompt or no tokens requested")
         if len(prompt) + max_new_tokens > self.gen.cache.max_len + 1:
             raise ValueError(f"request of {len(prompt)} + {max_new_tokens} tokens exceeds the cache "
                              f"({self.gen.cache.max_len})")
-        r = Request(list(prompt), max_new_tokens, eos_id)
+        if controls is not None:
+            controls.bias_row(self.gen.model.vocab_size)   # refuse a bad bias here, not when a slot becomes free
+        r = Request(list(prompt), max_new_tokens, eos_id, controls=controls)
         self.queue.append(r)
         return r
 
@@ -192,28 +232,41 @@ class ContinuousBatcher:
     @torch.no_grad()
     def step(self) -> list:
         """Admit, decode one token for every active sequence; returns the requests finished in this step."""
-        cache, finished = self.gen.cache, []
+        cache, finished = self.gen.cache, self._finished
         for i in range(len(self.slots)):
             if self.slots[i] is None and self.queue:
                 r = self.queue.pop(0)
+                if r.controls is not None:
+                    self._begin(i, r)
                 cache.reset_slot(i)
                 ids = torch.tensor([r.prompt], dtype=torch.long, device=self.gen.device)
                 logits = self.gen.model.forward_inference(ids, cache.slot(i))
+                if r.controls is not None:
+                    logits = self._proc(logits, row=i)
                 tok = int(Generator.sample(logits, self.temperature, self.top_k, self.rng)[0])
                 r._push(tok)
+                if r.controls is not None:
+                    self._proc.push_one(i, tok)
                 if r.done:
                     finished.append(r)
+                    self._release(i)
                 else:
                     self.slots[i] = r
                     self._next[i] = tok
         if self.active == 0:
-            return finished
+            return self._take_finished()
         for i, r in enumerate(self.slots):
             if r is None:
                 cache.reset_slot(i)
+            elif r.controls is not None:
+                self._restrict(i, r)
         logits = self.gen.decode(self._next)
+        if self._proc is not None:
+            logits = self._proc(logits)
         toks = Generator.sample(logits, self.temperature, self.top_k, self.rng)
         self._next.copy_(toks)
+        if self._proc is not None:
+            self._proc.push(toks)
         for i, t in enumerate(toks.tolist()):
             r = self.slots[i]
             if r is None:
@@ -221,8 +274,33 @@ class ContinuousBatcher:
             r._push(t)
             if r.done:
                 finished.append(r)
-                self.slots[i] = None
-        return finished
+                self._release(i)
+        return self._take_finished()
+
+    def _take_finished(self) -> list:
+        out, self._finished = self._finished, []
+        return out
+
+    def _begin(self, i: int, r: Request) -> None:
+        if self._proc is None:
+            self._proc = LogitProcessor(self.gen.batch, self.gen.cache.max_len + 1, self.gen.model.vocab_size,
+                                        self.gen.device)
+        self._proc.start(i, r.prompt, r.controls)
+        self._restrict(i, r)
+
+    def _restrict(self, i: int, r: Request) -> None:
+        """The next token's mask; a request whose grammar fails or allows nothing is dropped (its slot freed, ``done``
+        False) and the error raised, with every other request as it was."""
+        try:
+            self._proc.restrict(i, r.output)
+        except Exception:
+            self._release(i)
+            raise
+
+    def _release(self, i: int) -> None:
+        self.slots[i] = None
+        if self._proc is not None:
+            self._proc.stop(i)
 
     def run(self) -> list:
         """Serve until the queue is empty and every slot is idle; returns the requests in completion order."""

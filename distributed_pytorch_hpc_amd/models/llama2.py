@@ -166,6 +166,8 @@ class Attention(nn.Module):
         kernel over the cached prefix with the bottom-right causal mask."""
         if self.cp_attention is not None:
             raise NotImplementedError("KV-cache inference with context-parallel attention")
+        if cache.blocks is not None:
+            return self._cached_attention8(qkv, cos, sin, cache, cache.blocks[layer])
         b, s, _ = qkv.shape
         nh, nkv, hd = self.n_local_heads, self.n_local_kv_heads, self.head_dim
         kc, vc = cache.k[layer], cache.v[layer]
@@ -173,10 +175,7 @@ class Attention(nn.Module):
         if s == 1:
             return ops.decode_attention(qkv, kc, vc, cache.pos, nh, nkv, max_len=cache.attn_bound(),
                                         kv_scale=cache.kv_scale).view(b, 1, -1)
-        n = cache.length
-        if n is None:
-            raise RuntimeError("a multi-token append needs every sequence of the cache at the same, host-known length "
-                               "(prefill ragged prompts one sequence at a time through KVCache.slot)")
+        n = self._common_length(cache)
         q = qkv[:, :, : nh * hd].view(b, s, nh, hd)
         if not cache.fp8:
             o = ops.flash_attention(q, kc[:, : n + s], vc[:, : n + s], causal=True)
@@ -191,6 +190,36 @@ class Attention(nn.Module):
                 v = torch.cat([decode_ops.dequantize_kv(vc[:, :n], cache.kv_scale, v.dtype), v], 1)
             o = ops.flash_attention(q, k, v, causal=True)
         return o.reshape(b, s, nh * hd)
+
+    @staticmethod
+    def _common_length(cache: "KVCache") -> int:
+        n = cache.length
+        if n is None:
+            raise RuntimeError("a multi-token append needs every sequence of the cache at the same, host-known length "
+                               "(prefill ragged prompts one sequence at a time through KVCache.slot)")
+        return n
+
+    def _cached_attention8(self, qkv, cos, sin, cache: "KVCache", c8: ops.KV8Cache) -> torch.Tensor:
+        """``_cached_attention`` over a block-scaled 8-bit cache.  One new token attends over the cache as stored; several
+        attend over bf16 keys / values: their own (rotated in place in qkv by the append) after the prefix as it stood
+        before them, read back from the cache."""
+        b, s, _ = qkv.shape
+        nh, nkv, hd = self.n_local_heads, self.n_local_kv_heads, self.head_dim
+        if s == 1:
+            ops.kv8_append_(qkv, c8, cache.pos, cos, sin, nh, nkv)
+            return ops.kv8_decode_attention(qkv, c8, cache.pos, nh, nkv, max_len=cache.attn_bound()).view(b, 1, -1)
+        n = self._common_length(cache)
+        prefix = None
+        if n:   # before the append: it may store the open block's rows away
+            prefix = [torch.empty(b, n + s, nkv, hd, dtype=torch.bfloat16, device=qkv.device) for _ in range(2)]
+            ops.kv8_read(c8, cache.pos, n, tuple(x[:, :n] for x in prefix))
+        ops.kv8_append_(qkv, c8, cache.pos, cos, sin, nh, nkv)
+        q, k, v = decode_ops._split(qkv, nh, nkv, hd)
+        if prefix is not None:
+            for x, new in zip(prefix, (k, v)):
+                x[:, n:] = new
+            k, v = (x.to(qkv.dtype) for x in prefix)
+        return ops.flash_attention(q, k, v, causal=True).reshape(b, s, nh * hd)
 
 
 class FeedForward(nn.Module):
@@ -349,10 +378,13 @@ class KVCache:
     ``lengths`` mirrors pos on the host while it is known (None inside / after graph replays that the owner
     tracks itself).  ``slot(i)`` is a view of sequence i (prefill of prompts of different lengths).
     ``dtype=torch.float8_e4m3fn`` stores OCP e4m3 keys / values (value / ``kv_scale``): half the cache bytes.
+    ``kv_block=T`` (16 / 32 / 64 / 128) stores int8 (``dtype=torch.int8``) or e4m3 codes with a scale for every block of T
+    tokens of a KV head, taken from the block (ops.kv8): half the cache bytes without a scale to calibrate.  Its positions
+    only grow or restart at 0.
     Sized for HBM: 7B at 4 096 tokens is 2 GiB per sequence in bf16."""
 
     def __init__(self, model: "Transformer", batch: int, max_len: int, device=None, dtype: torch.dtype | None = None,
-                 kv_scale: float = 1.0):
+                 kv_scale: float = 1.0, kv_block: Optional[int] = None):
         args = model.model_args
         attn = model.layers[0].attention if len(model.layers) else None
         hkv = attn.n_local_kv_heads if attn is not None else args.kv_heads
@@ -362,14 +394,24 @@ class KVCache:
         if max_len > 2 * args.max_seq_len:
             raise ValueError(f"max_len {max_len} exceeds the RoPE table ({2 * args.max_seq_len} positions)")
         n_layers = max((layer.layer_id for layer in model.layers), default=-1) + 1   # pipeline stages keep ids
-        shape = (n_layers, batch, max_len, hkv, args.head_dim)
-        self.k = torch.zeros(shape, dtype=dtype, device=device)
-        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.blocks: Optional[list] = None   # per layer, with kv_block
+        if kv_block is not None:
+            if kv_scale != 1.0:
+                raise ValueError("KVCache: kv_block takes its scales from the blocks, kv_scale must stay 1")
+            self.blocks = [ops.kv8_cache(batch, max_len, hkv, args.head_dim, dtype, kv_block, device)
+                           for _ in range(n_layers)]
+            self.k, self.v = [c.k for c in self.blocks], [c.v for c in self.blocks]
+        elif dtype == torch.int8:
+            raise ValueError("KVCache: int8 entries need kv_block (tokens that share a scale)")
+        else:
+            shape = (n_layers, batch, max_len, hkv, args.head_dim)
+            self.k = torch.zeros(shape, dtype=dtype, device=device)
+            self.v = torch.zeros(shape, dtype=dtype, device=device)
         self.pos = torch.zeros(batch, dtype=torch.int32, device=device)
         self.batch, self.max_len = batch, max_len
         # dtype torch.float8_e4m3fn: OCP e4m3 entries holding key / kv_scale (half the bytes of bf16; decode is
         # bound by the cache read at large batch / long context)
-        self.fp8 = dtype == decode_ops.FP8_KV
+        self.fp8 = dtype == decode_ops.FP8_KV and kv_block is None
         self.kv_scale = float(kv_scale)
         self.lengths: Optional[list] = [0] * batch
         self._parent, self._index = None, None
@@ -404,7 +446,12 @@ class KVCache:
 
     def slot(self, i: int) -> "KVCache":
         view = object.__new__(KVCache)
-        view.k, view.v, view.pos = self.k[:, i:i + 1], self.v[:, i:i + 1], self.pos[i:i + 1]
+        view.pos = self.pos[i:i + 1]
+        if self.blocks is not None:
+            view.blocks = [c.slot(i) for c in self.blocks]
+            view.k, view.v = [c.k for c in view.blocks], [c.v for c in view.blocks]
+        else:
+            view.blocks, view.k, view.v = None, self.k[:, i:i + 1], self.v[:, i:i + 1]
         view.batch, view.max_len = 1, self.max_len
         view.fp8, view.kv_scale = self.fp8, self.kv_scale
         view.lengths = None if self.lengths is None else [self.lengths[i]]

@@ -21,7 +21,7 @@ sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."
 import torch  # noqa: E402
 import torch.distributed as dist  # noqa: E402
 
-from distributed_pytorch_hpc_amd.inference import Generator  # noqa: E402
+from distributed_pytorch_hpc_amd.inference import Generator, LogitControls  # noqa: E402
 from distributed_pytorch_hpc_amd.models.llama2 import build_llama, get_preset  # noqa: E402
 from distributed_pytorch_hpc_amd.parallel.tensor_parallel import parallelize_llama  # noqa: E402
 from distributed_pytorch_hpc_amd.train.cli import common_parser, finish, start  # noqa: E402
@@ -37,6 +37,9 @@ def main(argv=None):
     ap.add_argument("--max-new", type=int, default=32)
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-k", type=int, default=None)
+    ap.add_argument("--kv-dtype", choices=["model", "fp8", "int8"], default="model", help="KV-cache entries")
+    ap.add_argument("--kv-block", type=int, default=None, help="tokens that share a scale of an 8-bit cache (int8: 64)")
+    ap.add_argument("--repetition-penalty", type=float, default=1.0)
     ap.add_argument("--no-graphs", action="store_true", help="eager decode steps (default: HIP graphs on one GPU)")
     args = ap.parse_args(argv)
     rank, world, local, dev = start(args)
@@ -56,7 +59,9 @@ def main(argv=None):
     prompts = torch.randint(0, margs.vocab_size, (args.batch, args.prompt_len), generator=g)
 
     graphs = dev.type == "cuda" and world == 1 and not args.no_graphs
-    gen = Generator(model, args.batch, args.prompt_len + args.max_new, graphs=graphs)
+    kv_dtype = {"model": None, "fp8": torch.float8_e4m3fn, "int8": torch.int8}[args.kv_dtype]
+    gen = Generator(model, args.batch, args.prompt_len + args.max_new, graphs=graphs, dtype=kv_dtype,
+                    kv_block=args.kv_block or (64 if kv_dtype == torch.int8 else None))
     gen.generate(prompts, 2)   # warm-up: library set-up (and the graph capture on the first decode steps)
     sync = torch.cuda.synchronize if dev.type == "cuda" else (lambda: None)
     sync()
@@ -66,11 +71,20 @@ def main(argv=None):
     sync()
     t_prefill = time.perf_counter() - t0
     samp = torch.Generator(device=dev).manual_seed(args.seed) if args.temperature > 0 else None
-    tok = gen.sample(logits, args.temperature, args.top_k, samp)
+    controls = LogitControls(repetition_penalty=args.repetition_penalty)
+    proc = gen.processor(prompts.tolist(), controls if controls.penalizes else None)
+
+    def pick(logits):
+        tok = gen.sample(logits if proc is None else proc(logits), args.temperature, args.top_k, samp)
+        if proc is not None:
+            proc.push(tok)
+        return tok
+
+    tok = pick(logits)
     out = [tok]
     t1 = time.perf_counter()
     for _ in range(args.max_new - 1):
-        tok = gen.sample(gen.decode(tok), args.temperature, args.top_k, samp)
+        tok = pick(gen.decode(tok))
         out.append(tok)
     sync()
     t_decode = time.perf_counter() - t1
@@ -78,6 +92,7 @@ def main(argv=None):
     steps = max(args.max_new - 1, 1)
     summary = {"example": "generate_llama", "model": args.model, "tp": world, "batch": args.batch,
                "prompt_len": args.prompt_len, "new_tokens": args.max_new, "graphs": graphs,
+               "kv_dtype": args.kv_dtype, "repetition_penalty": args.repetition_penalty,
                "prefill_tokens_per_sec": args.batch * args.prompt_len / t_prefill,
                "decode_ms_per_step": 1000 * t_decode / steps,
                "decode_tokens_per_sec": args.batch * steps / t_decode,
