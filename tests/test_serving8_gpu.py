@@ -1,5 +1,5 @@
 """The serving loops over a block-scaled 8-bit cache with logit controls, on the MI355X: graph replays equal eager steps,
-batches equal single requests, logits stay close to the full forward."""
+logits stay close to the full forward, histories follow the tokens on the device."""
 import pytest
 import torch
 
@@ -57,9 +57,8 @@ def test_generate_graphed_equals_eager(dph_native, dtype):
     assert all((t % 3) == i % 3 for i, t in enumerate(eager[1][3:]))
 
 
-def test_continuous_batching_equals_single_requests(dph_native):
-    """Six requests on two slots, graphed, with and without controls; greedy ties aside, every one equals itself alone
-    (the batch changes how attention is split, so logits may differ in the last bits: compared on clear margins)."""
+def test_continuous_batching_graphed_equals_eager(dph_native):
+    """Six requests on two slots, with and without controls: a captured step gives what eager steps give."""
     from distributed_pytorch_hpc_amd.inference import ContinuousBatcher, Generator
 
     m = _tiny_llama(seed=9)
