@@ -318,7 +318,7 @@ struct Online {
 // The work of a call, in turns of 128 keys (32 for each wave of a workgroup): row (b, h, tile of 16 heads) has
 // ceil(n_b / 128) turns, at least one, and the rows' turns stand in one line, which the workgroups divide evenly whatever
 // the lengths are -- with a fixed number of keys a workgroup, sequences of 1000 to 4000 tokens left the card half idle at
-// the end (73 us against 5.5 TB/s at equal lengths).  The lengths are only known on the device, so every workgroup adds
+// the end (16 of 7B heads: 73 us, divided evenly 66).  The lengths are only known on the device, so every workgroup adds
 // them up for itself.
 struct Line {
   int turns;       // of all rows
@@ -385,7 +385,7 @@ __device__ __forceinline__ Line line_up(const KV8DecodeParams& p, int w) {
 }
 
 template <bool E4M3, int D>
-__global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
+__global__ __launch_bounds__(256, 2) void kv8_decode_k(KV8DecodeParams p) {
   constexpr int NI = D / 32, NE = D / 16, NH = D >= 64 ? D / 64 : 1, LD = D + 4;   // LD: rows of heads fall on other banks
   __shared__ float so[4][16][LD];
   __shared__ float sml[4][16][2];
@@ -402,57 +402,68 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
   // the d of chunk i of a key (and so of q) in the lanes of group g
   auto dof = [&](int i) { return D >= 64 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 8 * g; };
 
-  while (true) {   // one row's share of this workgroup's turns at a time: t0 .. t1 of nt
-    const int t1 = min(nt, t0 + stop - at);
-    const int h = p.tiles == 1 ? row : uni((unsigned)row / (unsigned)p.tiles), ct = row - h * p.tiles;
-    const int hq0 = h * G + ct * 16, nq = min(16, G - ct * 16);
-    const int full = n >> c.lgT << c.lgT;
-    bf16x8 qf[NI];   // q as the B operand: lane (head, g)
+  // A row's share of this workgroup's turns at a time: turns t0 .. t1 of nt.  What a share begins with -- q, its first
+  // keys, the scales of its first 64 blocks -- is asked for before the last share's sums are merged.
+  int t1, hq0, nq, full, end, first;
+  int64_t head;
+  bf16x8 qf[NI];              // q as the B operand: lane (head, g)
+  typename Raw<D>::K k[2][NH];
+  float ksl = 0.f, vsl = 0.f;   // lane i: the scales of block blk0 + i
+  int blk0 = 0, h;
+  // uniform base of a 16-key tile plus 32-bit offsets of the lane that stay the same; where the codes end with a step's
+  // first tile (T = 16), the second one re-reads it and is masked
+  const int ss = (int)c.c_ss;
+  const unsigned ko = (unsigned)(r16 * ss + (D >= 64 ? 16 : 8) * g);
+  unsigned vo[4];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      qf[i] = bf16x8{};
-      if (r16 < nq)
-        qf[i] = *reinterpret_cast<const bf16x8*>((const bf16*)p.q + (int64_t)b * p.q_sb + (int64_t)(hq0 + r16) * D + dof(i));
+  for (int j = 0; j < 4; ++j) vo[j] = (unsigned)((4 * g + j) * ss + r16 * NE);
+  auto tile = [&](int k0, int a) { return head + (int64_t)(k0 + (a && k0 + 16 < end ? 16 : 0)) * c.c_ss; };
+  auto load_k = [&](int k0) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const uint8_t* base = (const uint8_t*)c.kc + tile(k0, a);
+#pragma unroll
+      for (int x = 0; x < NH; ++x) k[a][x] = *reinterpret_cast<const typename Raw<D>::K*>(base + ko + 64 * x);
     }
+  };
+  auto load_scales = [&](int key) {
+    blk0 = key >> c.lgT;
+    if (blk0 + lane < end >> c.lgT) {
+      const int64_t off = (int64_t)b * c.s_sb + (int64_t)h * c.s_sh + (int64_t)(blk0 + lane) * c.s_sn;
+      ksl = c.ks[off];
+      vsl = c.vs[off];
+    }
+  };
+  auto begin = [&]() {
+    t1 = min(nt, t0 + stop - at);
+    h = p.tiles == 1 ? row : uni((unsigned)row / (unsigned)p.tiles);
+    const int ct = row - h * p.tiles;
+    hq0 = h * G + ct * 16;
+    nq = min(16, G - ct * 16);
+    full = n >> c.lgT << c.lgT;
+    end = t1 == nt ? full : 128 * t1;   // keys 128 t0 .. end are codes; a multiple of 16
+    first = 128 * t0 + 32 * wave;
+    head = (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
+    const bf16* q = (const bf16*)p.q + (int64_t)b * p.q_sb + (int64_t)(hq0 + min(r16, nq - 1)) * D;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) qf[i] = *reinterpret_cast<const bf16x8*>(q + dof(i));   // spare columns: the last head
+    if (first < end) {
+      load_scales(first);
+      load_k(first);
+    }
+  };
+  begin();
+  while (true) {
     Online<D> st;
     st.init();
-
-    const int end = t1 == nt ? full : 128 * t1;   // keys 128 t0 .. end are codes; a multiple of 16
-    const int first = 128 * t0 + 32 * wave;
     if (first < end) {
-      // spans of 64 blocks: lane i keeps the scales of the span's block i, so the loop over a span has no load of a
-      // single float (nor one under a condition, for which the compiler would wait with the loads of V in flight)
-      int blk0 = 0;
-      float ksl = 0.f, vsl = 0.f;
       auto scale_at = [&](float v, int key) {
         return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), (key >> c.lgT) - blk0));
       };
-      // uniform base of a 16-key tile plus 32-bit offsets of the lane that stay the same; where the codes end with the
-      // step's first tile (T = 16), the second one re-reads it and is masked
-      const int64_t head = (int64_t)b * c.c_sb + (int64_t)h * c.c_sh;
-      const int ss = (int)c.c_ss;
-      const unsigned ko = (unsigned)(r16 * ss + (D >= 64 ? 16 : 8) * g);
-      unsigned vo[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vo[j] = (unsigned)((4 * g + j) * ss + r16 * NE);
-      auto tile = [&](int k0, int a) { return head + (int64_t)(k0 + (a && k0 + 16 < end ? 16 : 0)) * c.c_ss; };
-      typename Raw<D>::K k[2][NH];
-      auto load_k = [&](int k0) {
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const uint8_t* base = (const uint8_t*)c.kc + tile(k0, a);
-#pragma unroll
-          for (int x = 0; x < NH; ++x) k[a][x] = *reinterpret_cast<const typename Raw<D>::K*>(base + ko + 64 * x);
-        }
-      };
-      load_k(first);
+      // spans of 64 blocks: the loop over a span has no load of a single float (nor one under a condition, for which the
+      // compiler would wait with the loads of V in flight)
       for (int span = first; span < end; span += 64 << c.lgT) {
-        blk0 = span >> c.lgT;
-        if (blk0 + lane < end >> c.lgT) {
-          const int64_t off = (int64_t)b * c.s_sb + (int64_t)h * c.s_sh + (int64_t)(blk0 + lane) * c.s_sn;
-          ksl = c.ks[off];
-          vsl = c.vs[off];
-        }
+        if (span != first) load_scales(span);
         const int span_end = min(end, span + (64 << c.lgT) - 127);
         for (int k0 = span; k0 < span_end; k0 += 128) {
           typename Raw<D>::V v[8];
@@ -491,24 +502,33 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
     // the open block's bf16 rows lie in the row's last turn (T divides 128): 32 of them a wave
     const int u0 = 32 * wave, rows = t1 == nt ? n - full : 0;
     if (u0 < rows) {
-      const bf16* kt = (const bf16*)c.kt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
-      const bf16* vt = (const bf16*)c.vt + (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
+      const int64_t base = (int64_t)b * c.t_sb + (int64_t)h * c.t_sh;
+      const char* kt = (const char*)((const bf16*)c.kt + base);
+      const char* vt = (const char*)((const bf16*)c.vt + base);
+      const unsigned ts = 2u * (unsigned)c.t_ss;
+      typedef __bf16 vrow __attribute__((ext_vector_type(NE)));
+      bf16x8 kr[2][NI];
+      vrow v[8];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const unsigned off = (unsigned)min(u0 + 16 * a + r16, rows - 1) * ts + 2u * (unsigned)dof(0);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) kr[a][i] = *reinterpret_cast<const bf16x8*>(kt + off + 2 * (dof(i) - dof(0)));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = *reinterpret_cast<const vrow*>(vt + (unsigned)min(u0 + 16 * (j >> 2) + 4 * g + (j & 3), rows - 1) * ts +
+                                              (unsigned)(r16 * NE * 2));
+      __builtin_amdgcn_sched_barrier(0);   // all sixteen loads before the first wait
       f32x4 s[2];
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         s[a] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const bf16* src = kt + (int64_t)min(u0 + 16 * a + r16, rows - 1) * c.t_ss;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) s[a] = mfma16(*reinterpret_cast<const bf16x8*>(src + dof(i)), qf[i], s[a]);
+        for (int i = 0; i < NI; ++i) s[a] = mfma16(kr[a][i], qf[i], s[a]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[a][r] = u0 + 16 * a + 4 * g + r < rows ? s[a][r] * sl2 : -INFINITY;
       }
-      typedef __bf16 vrow __attribute__((ext_vector_type(NE)));
-      vrow v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = *reinterpret_cast<const vrow*>(vt + (int64_t)min(u0 + 16 * (j >> 2) + 4 * g + (j & 3), rows - 1) * c.t_ss +
-                                              r16 * NE);
       const float one[2] = {1.f, 1.f};
       st.step(s, one, [&](int e) {
         bf16x8 o;
@@ -532,8 +552,7 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) so[wave][r16][NE * (4 * g + r) + e] = st.acc[e][r];
     }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == nt;
+    const bool whole = t0 == 0 && t1 == nt, none = n == 0;
     const int64_t slot = 2 * (int64_t)w + (t0 == 0 ? 1 : 0);   // one share that goes on from the last workgroup's row, one
                                                                // that the next one goes on with
     if (p.opart && t0 == 0 && tid == 0) {   // who has the row, for kv8_combine_k
@@ -541,7 +560,21 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
       info[0] = w;
       info[1] = owner_of(line, at + nt - 1) - w + 1;
     }
-    for (int i = tid; i < nq * D; i += 256) {
+    const int heads_here = nq;
+    const int64_t out_row = (int64_t)b * p.Hq + hq0;
+    at += t1 - t0;
+    const bool more = at < stop;
+    if (more) {
+      t0 = 0;
+      if (++row == heads) {
+        row = 0;
+        n = uni(length_of(p, ++b));
+        nt = turns_of(p, n);
+      }
+      begin();
+    }
+    __syncthreads();
+    for (int i = tid; i < heads_here * D; i += 256) {
       const int q = i / D, d = i % D;
       float M = -INFINITY, L = 0.f, o = 0.f;
 #pragma unroll
@@ -554,7 +587,7 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
         o = fmaf(a, so[x][q][d], o);
       }
       if (whole) {   // a sequence without keys has a zero output
-        ((bf16*)p.out)[((int64_t)b * p.Hq + hq0 + q) * D + d] = (bf16)(n > 0 ? o / L : 0.f);
+        ((bf16*)p.out)[(out_row + q) * D + d] = (bf16)(none ? 0.f : o / L);
       } else {
         p.opart[(slot * 16 + q) * D + d] = o;
         if (d == 0) {
@@ -563,15 +596,8 @@ __global__ __launch_bounds__(256, 3) void kv8_decode_k(KV8DecodeParams p) {
         }
       }
     }
-    at += t1 - t0;
-    if (at >= stop) break;
-    t0 = 0;
-    if (++row == heads) {
-      row = 0;
-      n = uni(length_of(p, ++b));
-      nt = turns_of(p, n);
-    }
-    __syncthreads();   // before the next row's sums overwrite these
+    if (!more) break;
+    __syncthreads();   // before the next share's sums overwrite these
   }
 }
 
@@ -713,7 +739,7 @@ void kv8_append(const KV8AppendParams& p, hipStream_t st) {
 }
 
 // Workgroups of a call: three to a CU (what the registers allow at once), or one for each turn that the longest sequences could have.
-int kv8_decode_workgroups(int64_t turns) { return (int)std::min<int64_t>(turns, 768); }
+int kv8_decode_workgroups(int64_t turns) { return (int)std::min<int64_t>(turns, 512); }
 
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t st) {
   const KV8& c = p.c;

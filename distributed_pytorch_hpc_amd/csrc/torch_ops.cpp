@@ -537,6 +537,7 @@ dph::KV8 check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const T
   TORCH_CHECK(strides_ok(kc, 16) && strides_ok(kt, 8),
               "kv8: head dim contiguous, the other strides multiples of 16 bytes");
   TORCH_CHECK(kc.stride(1) >= 0 && kc.stride(1) < (int64_t(1) << 26), "kv8: rows of k / v more than 64 MB apart");
+  TORCH_CHECK(kt.stride(1) >= 0 && kt.stride(1) < (int64_t(1) << 23), "kv8: rows of the tails more than 16 MB apart");
   check_align16(kc, "k"); check_align16(vc, "v"); check_align16(kt, "k_tail"); check_align16(vt, "v_tail");
   dph::KV8 c{};
   c.kc = kc.data_ptr(); c.vc = vc.data_ptr(); c.c_sb = kc.stride(0); c.c_ss = kc.stride(1); c.c_sh = kc.stride(2);
