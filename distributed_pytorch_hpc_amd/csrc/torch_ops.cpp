@@ -620,8 +620,8 @@ Tensor kv8_decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& v
   return out;
 }
 
-void kv8_read_(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& kt,
-               const Tensor& vt, const Tensor& pos, Tensor& ko, Tensor& vo) {
+void kv8_read_into(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& kt,
+                   const Tensor& vt, const Tensor& pos, Tensor& ko, Tensor& vo) {
   dph::KV8ReadParams p{};
   p.c = check_kv8(kc, vc, ks, vs, kt, vt);
   c10::DeviceGuard g(kc.device());
@@ -633,7 +633,6 @@ void kv8_read_(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tenso
   TORCH_CHECK(ko.size(1) <= p.c.Smax, "kv8_read: count ", ko.size(1), " exceeds the cache's ", p.c.Smax, " rows");
   TORCH_CHECK(strides_ok(ko, 8), "kv8_read: outputs need a contiguous head dim and strides that are multiples of 8");
   check_align16(ko, "k_out"); check_align16(vo, "v_out");
-  no_overlap({&ko, &vo});
   TORCH_CHECK(int64_t(p.c.B) * p.c.Hkv * 2 * (ko.size(1) * p.c.D / 8192 + 1) < (int64_t(1) << 24),
               "kv8_read: too large for one launch");
   p.pos = pos.data_ptr<int>();
@@ -642,13 +641,21 @@ void kv8_read_(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tenso
   dph::kv8_read(p, cur_stream());
 }
 
+void kv8_read_(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& kt,
+               const Tensor& vt, const Tensor& pos, Tensor& ko, Tensor& vo) {
+  no_overlap({&ko, &vo});
+  for (const Tensor* o : {&ko, &vo})
+    for (const Tensor* t : {&kc, &vc, &ks, &vs, &kt, &vt}) at::assert_no_overlap(*o, *t);
+  kv8_read_into(kc, vc, ks, vs, kt, vt, pos, ko, vo);
+}
+
 std::tuple<Tensor, Tensor> kv8_read(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
                                     const Tensor& kt, const Tensor& vt, const Tensor& pos, int64_t count) {
   TORCH_CHECK(kc.dim() == 4 && count >= 0 && count <= kc.size(1), "kv8_read: count ", count, " is not in 0 .. Smax");
   c10::DeviceGuard g(kc.device());
   auto ko = at::empty({kc.size(0), count, kc.size(2), kc.size(3)}, kc.options().dtype(at::kBFloat16));
   auto vo = at::empty(ko.sizes(), ko.options());
-  kv8_read_(kc, vc, ks, vs, kt, vt, pos, ko, vo);
+  kv8_read_into(kc, vc, ks, vs, kt, vt, pos, ko, vo);
   return {ko, vo};
 }
 

@@ -376,3 +376,91 @@ def test_offsets_past_32_bits(dph_native):
     assert torch.equal(got[-1:], ops.kv8_decode_attention(one[-1:], small, pos[-1:].clone(), hq, hkv))
     k, v = ops.kv8_read(c.slot(batch - 1), pos[-1:].clone() + 1, 120)
     assert torch.equal(v[0, -100:].cpu(), ops.kv8_read(ref, _pos(cap), 100)[1][0])
+
+
+def test_read_refuses_outputs_over_the_cache(dph_native):
+    ops = _ops()
+    c = ops.kv8_cache(2, 40, 2, 32, block=16, device=DEV)
+    pos = _pos(3, 5).to(DEV)
+    a = torch.zeros(2, 4, 2, 32, dtype=torch.bfloat16, device=DEV)
+    for out in ((a, a), (c.k_tail[:, :4], a), (a, a.clone()[:1].expand(2, -1, -1, -1))):
+        with pytest.raises(RuntimeError):
+            ops.kv8_read(c, pos, 4, out)
+
+
+def test_no_sequences_and_no_tokens(dph_native):
+    ops = _ops()
+    cos, sin = tables(32, 40, DEV)
+    c = ops.kv8_cache(0, 40, 2, 32, block=16, device=DEV)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    ops.kv8_append_(torch.zeros(0, 3, 256, dtype=torch.bfloat16, device=DEV), c, none, cos, sin, 4, 2)
+    one = torch.zeros(0, 1, 256, dtype=torch.bfloat16, device=DEV)
+    assert ops.kv8_decode_attention(one, c, none, 4, 2).shape == (0, 128)
+    assert ops.kv8_read(c, none, 7)[1].shape == (0, 7, 2, 32)
+    c = _to(filled(ops.kv8_cache(2, 40, 2, 32, block=16), 1), DEV)
+    before = type(c)(*(t.clone() for t in c))
+    ops.kv8_append_(torch.zeros(2, 0, 256, dtype=torch.bfloat16, device=DEV), c, _pos(3, 5).to(DEV), cos, sin, 4, 2)
+    _same(c, before)
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65, 130])
+def test_decode_attention_many_sequences(dph_native, batch):
+    """Lengths from none to the capacity, more sequences than lanes: every one equals itself in a batch of one, up to how
+    its sum is divided (compared with the oracle)."""
+    ops = _ops()
+    hq, hkv, d, t, cap = 4, 2, 32, 16, 700
+    c = _to(filled(ops.kv8_cache(batch, cap, hkv, d, block=t), 15), DEV)
+    pos = (torch.arange(batch) * 37 % (cap + 1) - 1).int()
+    qkv = make_qkv(batch, 1, hq, hkv, d, 16, DEV)
+    got = ops.kv8_decode_attention(qkv, c, pos.to(DEV), hq, hkv)
+    some = [0, 1, batch // 2, batch - 2, batch - 1]
+    small = type(c)(*(x[some] for x in c))
+    want, off = attention64(qkv[some], small, pos[some], hq, hkv, d ** -0.5)
+    assert_close64(got[some], want, off)
+    for i in range(batch):   # the kernel's own sums of one sequence, one rounding of each side apart
+        alone = ops.kv8_decode_attention(qkv[i:i + 1], c.slot(i), pos[i:i + 1].to(DEV), hq, hkv)
+        torch.testing.assert_close(got[i:i + 1].float(), alone.float(), rtol=2 * 2.0 ** -8, atol=2.0 ** -12)
+
+
+@pytest.mark.parametrize("max_len", [1, 100, 128, 129, 333])
+def test_decode_attention_max_len_only_splits_the_work(dph_native, max_len):
+    """A bound that is too low, too high or right gives the same attention."""
+    ops = _ops()
+    c = _to(filled(ops.kv8_cache(4, 333, 2, 64, block=32), 18), DEV)
+    pos = _pos(-1, 40, 128, 332).to(DEV)
+    qkv = make_qkv(4, 1, 6, 2, 64, 19, DEV)
+    want, off = attention64(qkv, c, pos, 6, 2, 0.125)
+    assert_close64(ops.kv8_decode_attention(qkv, c, pos, 6, 2, scale=0.125, max_len=max_len), want, off)
+
+
+def test_decode_attention_past_the_capacity(dph_native):
+    """Positions at and past Smax (a replayed graph run too far) see the rows that exist."""
+    ops = _ops()
+    c = _to(filled(ops.kv8_cache(3, 70, 2, 64, block=32), 21), DEV)
+    pos = _pos(69, 70, 2 ** 31 - 1).to(DEV)
+    qkv = make_qkv(1, 1, 4, 2, 64, 22, DEV).expand(3, -1, -1)
+    same = type(c)(*(x[:1].expand_as(x).contiguous() for x in c))
+    got = ops.kv8_decode_attention(qkv, same, pos, 4, 2)
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    for a, b in zip(ops.kv8_read(same, pos + torch.tensor([1, 0, 0], device=DEV, dtype=torch.int32), 30), range(2)):
+        assert torch.equal(a[0], a[1]) and torch.equal(a[0], a[2])
+
+
+def test_decode_attention_scales_far_apart(dph_native):
+    """One block of V 2^-40 of the others' size with all of the weight on it: its digits are not lost."""
+    ops = _ops()
+    hq, hkv, d, t, n = 2, 2, 128, 16, 600
+    c = _to(filled(ops.kv8_cache(1, n, hkv, d, block=t), 23), DEV)
+    c.v_scale[:, 20] *= 2.0 ** -40
+    c.k_scale[:, :20] *= 1e-3
+    c.k_scale[:, 21:] *= 1e-3
+    c.k[:, 20 * t:21 * t] = 64
+    c.k_scale[:, 20] = 1.0
+    c.k_tail.mul_(1e-3)
+    qkv = make_qkv(1, 1, hq, hkv, d, 24, DEV)
+    qkv[:, :, :hq * d] = 1.0
+    pos = _pos(n - 1).to(DEV)
+    want, off = attention64(qkv, c, pos, hq, hkv, d ** -0.5)
+    got = ops.kv8_decode_attention(qkv, c, pos, hq, hkv)
+    assert float(want.abs().max()) < 2.0 ** -36
+    assert_close64(got, want, off)
