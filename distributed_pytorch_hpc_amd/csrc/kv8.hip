@@ -158,6 +158,7 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
     unsigned mx = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
+      if (i * 256 + tid >= chunks) continue;   // not its chunk: the owner may have rotated it in qkv before it was read
       const u32x4 u = __builtin_bit_cast(u32x4, val[i]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) mx = max(mx, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));

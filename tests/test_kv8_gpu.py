@@ -97,6 +97,23 @@ def test_append_bitwise(dph_native, code, hq, hkv, d, t, s):
     _same(got, ref)
 
 
+@pytest.mark.parametrize("hkv,d,t", [(8, 32, 16), (4, 64, 16), (8, 32, 32), (2, 32, 64)])
+def test_append_bitwise_many_small_blocks(dph_native, hkv, d, t):
+    """Blocks of fewer chunks than a workgroup has threads: the spare threads, which read a chunk that its owner rotates in
+    place meanwhile, have no part in the scale."""
+    ops = _ops()
+    s, cap = 900, 960
+    qkv = make_qkv(6, s, hkv, hkv, d, 12, "cpu")
+    ref = ops.kv8_cache(6, cap, hkv, d, block=t)
+    got, x = _to(ref, DEV), qkv.to(DEV)
+    cos, sin = tables(d, cap, "cpu")
+    pos = _pos(0, 1, 15, 16, 40, 60)
+    ops.kv8_append_(qkv, ref, pos, cos, sin, hkv, hkv)
+    ops.kv8_append_(x, got, pos.to(DEV), cos.to(DEV), sin.to(DEV), hkv, hkv)
+    _equal(x, qkv)
+    _same(got, ref)
+
+
 @pytest.mark.parametrize("code", CODES)
 def test_append_values_at_the_edges(dph_native, code):
     """Blocks of zeros, of the least and the largest bf16 numbers, and with infinities or NaN."""
