@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from dist_utils import run_distributed
 from test_inference import _model
 
 CODES = [torch.int8, torch.float8_e4m3fn]
@@ -172,3 +173,23 @@ def test_temperature_sampling_stays_inside_the_mask():
     out = Generator(m, 2, 32).generate([[1], [2, 3]], 20, temperature=2.0, top_k=10, controls=LogitControls(allowed=lambda _: few),
                                        generator=torch.Generator().manual_seed(0))
     assert set(out[0][1:]) | set(out[1][2:]) <= {3, 50, 96}
+
+
+def _tp_worker(rank, world):
+    import torch.distributed as dist
+
+    from distributed_pytorch_hpc_amd.inference import Generator, LogitControls
+    from distributed_pytorch_hpc_amd.parallel.tensor_parallel import parallelize_llama
+
+    m = _model(vocab=96)
+    if world > 1:
+        parallelize_llama(m, dist.group.WORLD, sequence_parallel=False, loss_parallel=False)
+    return Generator(m, 2, 40, dtype=torch.int8, kv_block=16).generate(
+        [[1, 2, 3, 4, 5], [7, 8, 9, 10, 11]], 20, controls=LogitControls(repetition_penalty=1.3, frequency_penalty=0.1))
+
+
+def test_tensor_parallel_block_scaled_cache_with_controls():
+    """A scale belongs to one KV head, so sharding the heads over two ranks changes neither codes nor tokens."""
+    ref = _tp_worker(0, 1)
+    for out in run_distributed(_tp_worker, 2):
+        assert out == ref
