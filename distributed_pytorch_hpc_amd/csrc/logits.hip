@@ -5,7 +5,7 @@
 // atomics, so the order of arrival does not matter -- between asking for its logits and using them.  No state is kept from
 // call to call: reading the ids again costs 8 bytes a token of the history, a [N, V] table of counts 4 bytes a logit.
 // Bound by latency (launch, ids, LDS) and then by memory: one row of 32 000 with 300 ids 3.4 us; 64 rows, bf16, 4000 ids
-// each, bias and mask 7.9 us, 2.4 TB/s of its 19 MB; 64 rows of fp32 with a mask alone 6.2 us.  Loads under conditions of
+// each, bias and mask 7.1 us, 2.6 TB/s of its 19 MB; 64 rows of fp32 with a mask alone 6.2 us.  Loads under conditions of
 // their own, each waiting for the last, took 23 us.
 #include "dph_common.h"
 #include "kernels.h"
@@ -35,14 +35,12 @@ __device__ __forceinline__ void put<float, 8>(Chunk<float, 8>& c, int e, float v
   else c.b[e - 4] = v;
 }
 
-// 8 logits a thread, in one chunk where every row begins at 16 bytes (CH = 8), else one by one.  Segments of 2048: longer
-// ones read the history less often but wait for their own tail (4096: 9.0, 2048: 8.4 us at 64 x 32 000, 4000 ids a row).
-constexpr int kSeg = 2048;
-template <typename T, int CH>
-__global__ __launch_bounds__(256) void process_logits_k(LogitParams p, int nseg) {
-  constexpr int NC = kSeg / 256 / CH;
-  __shared__ __align__(16) unsigned cnt[kSeg];
-  const int row = blockIdx.x / nseg, v0 = blockIdx.x % nseg * kSeg, nv = min(kSeg, p.V - v0);
+// 8 logits a thread, in one chunk where every row begins at 16 bytes (CH = 8), else one by one: a segment of 8 * NT.
+template <typename T, int CH, int NT>
+__global__ __launch_bounds__(NT) void process_logits_k(LogitParams p, int nseg) {
+  constexpr int NC = 8 / CH, SEG = 8 * NT;
+  __shared__ __align__(16) unsigned cnt[SEG];
+  const int row = blockIdx.x / nseg, v0 = blockIdx.x % nseg * SEG, nv = min(SEG, p.V - v0);
   const int tid = threadIdx.x;
   const T* x = (const T*)p.x + (int64_t)row * p.ldx + v0;
   T* y = (T*)p.y + (int64_t)row * p.V + v0;
@@ -51,7 +49,7 @@ __global__ __launch_bounds__(256) void process_logits_k(LogitParams p, int nseg)
   Chunk<T, CH> xr[NC];
   Chunk<float, CH> br[NC];
   int mr[NC];
-  auto at = [&](int k) { return min((k * 256 + tid) * CH, nv - CH); };
+  auto at = [&](int k) { return min((k * NT + tid) * CH, nv - CH); };
 #pragma unroll
   for (int k = 0; k < NC; ++k) xr[k] = *reinterpret_cast<const Chunk<T, CH>*>(x + at(k));
   if (p.mask) {
@@ -67,7 +65,7 @@ __global__ __launch_bounds__(256) void process_logits_k(LogitParams p, int nseg)
   float rep = 1.f, inv = 1.f, f = 0.f, a = 0.f;
   if (p.tokens) {
     const u32x4 zero = {0, 0, 0, 0};
-    for (int i = tid; i < kSeg / 4; i += 256) *reinterpret_cast<u32x4*>(&cnt[4 * i]) = zero;
+    for (int i = tid; i < SEG / 4; i += NT) *reinterpret_cast<u32x4*>(&cnt[4 * i]) = zero;
     const int len = max(0, min(p.lengths[row], p.L)), plen = p.prompt ? p.prompt[row] : 0;
     if (p.rep) {
       rep = p.rep[row];
@@ -77,15 +75,15 @@ __global__ __launch_bounds__(256) void process_logits_k(LogitParams p, int nseg)
     if (p.pres) a = p.pres[row];
     const int64_t* ids = p.tokens + (int64_t)row * p.ldt;
     __syncthreads();
-    for (int i0 = tid; i0 < len; i0 += 256 * 8) {   // eight loads in flight
+    for (int i0 = tid; i0 < len; i0 += NT * 8) {   // eight loads in flight
       int64_t id[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) id[u] = ids[min(i0 + 256 * u, len - 1)];
+      for (int u = 0; u < 8; ++u) id[u] = ids[min(i0 + NT * u, len - 1)];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int64_t o = id[u] - v0;   // ids outside the vocabulary (padding) fall into no segment
-        if (i0 + 256 * u < len && o >= 0 && o < nv) {
-          if (i0 + 256 * u < plen) atomicOr(&cnt[o], kInPrompt);
+        if (i0 + NT * u < len && o >= 0 && o < nv) {
+          if (i0 + NT * u < plen) atomicOr(&cnt[o], kInPrompt);
           else atomicAdd(&cnt[o], 1u);
         }
       }
@@ -94,7 +92,7 @@ __global__ __launch_bounds__(256) void process_logits_k(LogitParams p, int nseg)
   }
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
-    const int i = (k * 256 + tid) * CH;
+    const int i = (k * NT + tid) * CH;
     if (i >= nv) continue;
     const unsigned allowed = p.mask ? (unsigned)mr[k] >> ((v0 + i) & 31) : ~0u;
     Chunk<T, CH> o;
@@ -123,15 +121,29 @@ void process_logits(const LogitParams& p, int dtype, hipStream_t st) {
   };
   const int es = dtype == kBF16 ? 2 : 4;
   const bool vec = p.V % 8 == 0 && aligned(p.x, p.ldx, es) && aligned(p.bias, p.ldb, 4);
-  const int nseg = (int)cdiv(p.V, kSeg);
-  const dim3 grid((unsigned)((int64_t)nseg * p.N));
-#define DPH_LOGITS(T_)                                                                                          \
-  do {                                                                                                          \
-    if (vec) hipLaunchKernelGGL((process_logits_k<T_, 8>), grid, dim3(256), 0, st, p, nseg);                    \
-    else hipLaunchKernelGGL((process_logits_k<T_, 1>), grid, dim3(256), 0, st, p, nseg);                        \
+  // Every segment of a row reads the whole history: with 1024 threads there are a quarter as many, but few rows fill the
+  // card worse and a workgroup waits for more.  Measured (us, 256 / 1024 threads, bf16, bias and mask, V = 32 000):
+  //   1 row:   300 ids 3.4 / 4.6,  4000 4.3 / 5.0,  8000 5.0 / 5.1,  32 768 10.9 / 7.8
+  //   16 rows: 300 ids 3.6 / 4.6,  4000 4.6 / 5.2,  8000 6.2 / 5.3,  32 768 16.3 / 8.5
+  //   64 rows: 300 ids 6.4 / 5.9,  4000 8.2 / 7.1,  8000 10.2 / 7.7, 32 768 22.6 / 14.4
+  // and 64 rows without a history 6.2 / 6.4.
+  const bool wide = p.tokens && (p.L >= 6144 || (int64_t)p.N * p.V >= 3 << 19);
+#define DPH_LOGITS(T_, CH_, NT_)                                                                                       \
+  do {                                                                                                                 \
+    const int nseg = (int)cdiv(p.V, 8 * NT_);                                                                          \
+    hipLaunchKernelGGL((process_logits_k<T_, CH_, NT_>), dim3((unsigned)((int64_t)nseg * p.N)), dim3(NT_), 0, st, p,   \
+                       nseg);                                                                                          \
   } while (0)
-  if (dtype == kBF16) DPH_LOGITS(bf16);
-  else DPH_LOGITS(float);
+#define DPH_LOGITS_T(T_)                                      \
+  do {                                                        \
+    if (vec && wide) DPH_LOGITS(T_, 8, 1024);                 \
+    else if (vec) DPH_LOGITS(T_, 8, 256);                     \
+    else if (wide) DPH_LOGITS(T_, 1, 1024);                   \
+    else DPH_LOGITS(T_, 1, 256);                              \
+  } while (0)
+  if (dtype == kBF16) DPH_LOGITS_T(bf16);
+  else DPH_LOGITS_T(float);
+#undef DPH_LOGITS_T
 #undef DPH_LOGITS
 }
 
