@@ -193,3 +193,19 @@ def test_tensor_parallel_block_scaled_cache_with_controls():
     ref = _tp_worker(0, 1)
     for out in run_distributed(_tp_worker, 2):
         assert out == ref
+
+
+def test_example_runs_with_block_scaled_cache_and_penalty():
+    import json
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, os.path.join(root, "examples", "08_serving", "generate_llama.py"), "--model",
+                          "tiny", "--batch", "2", "--prompt-len", "20", "--max-new", "18", "--kv-dtype", "int8",
+                          "--kv-block", "16", "--repetition-penalty", "1.3"], capture_output=True, text=True, timeout=300,
+                         env=dict(os.environ, MASTER_ADDR="127.0.0.1"))
+    assert out.returncode == 0, out.stderr[-2000:]
+    s = json.loads([ln for ln in out.stdout.splitlines() if ln.startswith("{")][-1])
+    assert s["kv_dtype"] == "int8" and len(s["first_sequence_new_ids"]) == 16
