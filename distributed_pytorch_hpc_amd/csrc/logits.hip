@@ -127,7 +127,9 @@ void process_logits(const LogitParams& p, int dtype, hipStream_t st) {
   //   16 rows: 300 ids 3.6 / 4.6,  4000 4.6 / 5.2,  8000 6.2 / 5.3,  32 768 16.3 / 8.5
   //   64 rows: 300 ids 6.4 / 5.9,  4000 8.2 / 7.1,  8000 10.2 / 7.7, 32 768 22.6 / 14.4
   // and 64 rows without a history 6.2 / 6.4.
-  const bool wide = p.tokens && (p.L >= 6144 || (int64_t)p.N * p.V >= 3 << 19);
+  // A grid holds fewer than 2^32 threads: rows too many for 1024 each (the caller bounds N for 256) take the narrow form.
+  const bool wide = p.tokens && (p.L >= 6144 || (int64_t)p.N * p.V >= 3 << 19) &&
+                    (int64_t)p.N * cdiv(p.V, 8 * 1024) < int64_t(1) << 22;
 #define DPH_LOGITS(T_, CH_, NT_)                                                                                       \
   do {                                                                                                                 \
     const int nseg = (int)cdiv(p.V, 8 * NT_);                                                                          \

@@ -163,3 +163,16 @@ def test_graph_replays(dph_native):
         assert torch.equal(y, ops.process_logits(xd, td, ld, **kd))
         ld += 5
         torch.cuda.synchronize()
+
+
+def test_more_rows_than_wide_workgroups(dph_native):
+    """2^22 + 1 rows of four tokens with a history each: 1024 threads a row would be more than a launch takes.  Integers,
+    so the result is exact."""
+    ops = _ops()
+    n = 2 ** 22 + 1
+    x = (torch.arange(4 * n, device=DEV) % 97).float().view(n, 4)
+    tokens = (torch.arange(n, device=DEV) % 4)[:, None]
+    got = ops.process_logits(x, tokens, torch.ones(n, dtype=torch.int32, device=DEV),
+                             presence=(torch.arange(n, device=DEV) % 5).float())
+    want = x.scatter_add(1, tokens, -(torch.arange(n, device=DEV) % 5).float()[:, None])
+    assert torch.equal(got, want)
