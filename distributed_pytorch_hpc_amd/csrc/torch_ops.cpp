@@ -4,6 +4,7 @@
 // launch, so a kernel never sees a layout it was not written for.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -514,6 +515,14 @@ bool strides_ok(const Tensor& t, int64_t mult) {   // unit stride along the last
   return true;
 }
 
+// Operators without a backward refuse to cut a graph silently (checked here: nine looks at a tensor cost 1 us in Python)
+void refuse_grad(const char* name, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), name, " has no backward: call it under torch.no_grad() or on "
+                "detached tensors");
+}
+
 dph::KV8 check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& kt,
                    const Tensor& vt) {
   TORCH_CHECK(kc.is_cuda() && kc.dim() == 4 && kt.dim() == 4 && ks.dim() == 3, "kv8: k / v [B, Smax, Hkv, D], scales "
@@ -568,6 +577,7 @@ void no_overlap(std::initializer_list<const Tensor*> ts) {   // written operands
 
 void kv8_append_(Tensor& qkv, Tensor& kc, Tensor& vc, Tensor& ks, Tensor& vs, Tensor& kt, Tensor& vt, const Tensor& pos,
                  const Tensor& cos, const Tensor& sin, int64_t n_heads, int64_t n_kv_heads) {
+  refuse_grad("kv8_append_", {&qkv, &kc, &vc, &ks, &vs, &kt, &vt, &cos, &sin});
   dph::KV8AppendParams p{};
   p.c = check_kv8(kc, vc, ks, vs, kt, vt);
   c10::DeviceGuard g(kc.device());
@@ -592,6 +602,7 @@ void kv8_append_(Tensor& qkv, Tensor& kc, Tensor& vc, Tensor& ks, Tensor& vs, Te
 Tensor kv8_decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
                             const Tensor& kt, const Tensor& vt, const Tensor& pos, int64_t n_heads, int64_t n_kv_heads,
                             double scale, int64_t max_len) {
+  refuse_grad("kv8_decode_attention", {&qkv, &kc, &vc, &ks, &vs, &kt, &vt});
   dph::KV8DecodeParams p{};
   p.c = check_kv8(kc, vc, ks, vs, kt, vt);
   c10::DeviceGuard g(kc.device());
@@ -622,6 +633,7 @@ Tensor kv8_decode_attention(const Tensor& qkv, const Tensor& kc, const Tensor& v
 
 void kv8_read_into(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& kt,
                    const Tensor& vt, const Tensor& pos, Tensor& ko, Tensor& vo) {
+  refuse_grad("kv8_read", {&kc, &vc, &ks, &vs, &kt, &vt, &ko, &vo});
   dph::KV8ReadParams p{};
   p.c = check_kv8(kc, vc, ks, vs, kt, vt);
   c10::DeviceGuard g(kc.device());
@@ -665,6 +677,9 @@ Tensor process_logits(const Tensor& logits, const c10::optional<Tensor>& tokens,
                       const c10::optional<Tensor>& bias, const c10::optional<Tensor>& mask) {
   check_cuda(logits, "logits");
   c10::DeviceGuard g(logits.device());
+  refuse_grad("process_logits", {&logits});
+  for (const auto* t : {&repetition, &presence, &frequency, &bias})
+    if (t->has_value()) refuse_grad("process_logits", {&**t});
   TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
               "process_logits: logits must be [N, V] with a contiguous last dim");
   const int64_t N = logits.size(0), V = logits.size(1);

@@ -65,7 +65,7 @@ def kv8_cache(batch: int, max_len: int, n_kv_heads: int, head_dim: int, dtype: t
 
 
 def _no_grad(name: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
@@ -180,6 +180,7 @@ def kv8_append_(qkv: torch.Tensor, cache: KV8Cache, pos: torch.Tensor, cos: torc
     if _lib.use_native(qkv):
         _lib.ops().kv8_append_(qkv, *cache, pos, cos, sin, n_heads, n_kv_heads)
         return
+    _no_grad("kv8_append_", *cache, cos, sin)
     _check(cache, pos, qkv, n_heads, n_kv_heads, (cos, sin))
     kv8_append_reference(qkv, cache, pos, cos, sin, n_heads, n_kv_heads)
 
@@ -194,6 +195,7 @@ def kv8_decode_attention(qkv: torch.Tensor, cache: KV8Cache, pos: torch.Tensor, 
     if _lib.use_native(qkv):
         return _lib.ops().kv8_decode_attention(qkv, *cache, pos, n_heads, n_kv_heads, scale,
                                                cache.k.shape[1] if max_len is None else max_len)
+    _no_grad("kv8_decode_attention", *cache)
     _check(cache, pos, qkv, n_heads, n_kv_heads)
     if qkv.shape[1] != 1:
         raise ValueError("kv8_decode_attention: one token per sequence (qkv [B, 1, ...])")
@@ -213,6 +215,7 @@ def kv8_read(cache: KV8Cache, pos: torch.Tensor, count: int,
             raise ValueError(f"kv8_read: out must be two [B, {count}, Hkv, D] tensors")
         _lib.ops().kv8_read_(*cache, pos, *out)
         return out
+    _no_grad("kv8_read", *cache, *(out or ()))
     _check(cache, pos)
     if not 0 <= count <= cache.k.shape[1]:
         raise ValueError(f"kv8_read: count {count} is not in 0 .. {cache.k.shape[1]}")

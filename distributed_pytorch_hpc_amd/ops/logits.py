@@ -85,11 +85,13 @@ def process_logits(logits: torch.Tensor, tokens: Opt = None, lengths: Opt = None
     tokens int64 [N, L], lengths / prompt_lengths int32 [N] (ids outside 0 .. V - 1 are ignored; without prompt_lengths
     every id counts as generated), repetition / presence / frequency fp32 [N], bias fp32 [V] or [N, V], mask int32
     [ceil(V / 32)] or [N, ceil(V / 32)] (``pack_token_mask``).  Anything may be None.  A row whose mask allows nothing
-    comes back as -inf throughout.  No backward: logits that require grad are refused."""
+    comes back as -inf throughout.  No backward: operands that require grad are refused."""
     if torch.is_grad_enabled() and logits.requires_grad:
         raise RuntimeError("process_logits has no backward: call it under torch.no_grad() or on detached logits")
     if _lib.use_native(logits):
         return _lib.ops().process_logits(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias,
                                          mask)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (repetition, presence, frequency, bias)):
+        raise RuntimeError("process_logits has no backward: call it under torch.no_grad() or on detached tensors")
     _check(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias, mask)
     return process_logits_reference(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias, mask)
