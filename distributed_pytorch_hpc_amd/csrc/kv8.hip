@@ -270,6 +270,16 @@ __device__ __forceinline__ bf16x8 column(const V (&v)[8], int e) {
 // 2^x, zero below 2^-126: a weight that small adds nothing
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+__device__ __forceinline__ bf16x8 finite_or_zero(bf16x8 v) {
+  u32x4 u = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const unsigned x = u[k];
+    u[k] = ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u) | ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu);
+  }
+  return __builtin_bit_cast(bf16x8, u);
+}
+
 // The running softmax of one wave: lane (c, g) holds head c's maximum, its own keys' share of the sum, and rows
 // (D / 16) (4 g + r) + e of O^T in acc[e][r].
 template <int D>
@@ -282,8 +292,11 @@ struct Online {
     m = -INFINITY;
     l = 0.f;
   }
-  // s: scores in units of log2 (-inf: no key); vs: scale of V of the two tiles; column(e): A operand of d-tile e
-  template <typename F>
+  // s: scores in units of log2 (-inf: no key); vs: scale of V of the two tiles; column(e): A operand of d-tile e.
+  // OPEN: V is bf16 and may hold infinities (codes have none, a block with one has the scale NaN).  The weight's low part
+  // is zero or of either sign, so it must not meet them: their sum with the high part alone is the infinity that stands
+  // there.  A sum that is finite has met none; looking at the sums takes 0.1 to 0.2 us of a call, less than looking at V.
+  template <bool OPEN, typename F>
   __device__ __forceinline__ void step(const f32x4 (&s)[2], const float (&vs)[2], F&& vcol) {
     float mx = m;
 #pragma unroll
@@ -312,11 +325,28 @@ struct Online {
         hi[4 * a + r] = h;
         lo[4 * a + r] = (bf16)(w - (float)h);
       }
+    if constexpr (OPEN) {
+      float z = 0.f;
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) {
-      const bf16x8 v = vcol(e);
-      acc[e] = mfma16(v, hi, acc[e]);
-      acc[e] = mfma16(v, lo, acc[e]);
+      for (int e = 0; e < D / 16; ++e) {
+        acc[e] = mfma16(vcol(e), hi, acc[e]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z = fmaf(acc[e][r], 0.f, z);
+      }
+      const bool finite = !__any(z != 0.f);
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) {
+        bf16x8 v = vcol(e);
+        if (!finite) v = finite_or_zero(v);
+        acc[e] = mfma16(v, lo, acc[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) {
+        const bf16x8 v = vcol(e);
+        acc[e] = mfma16(v, hi, acc[e]);
+        acc[e] = mfma16(v, lo, acc[e]);
+      }
     }
   }
 };
@@ -501,7 +531,7 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_k(KV8DecodeParams p) {
           }
           if (k0 + 16 >= end) s[1] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           load_k(k0 + 128 < end ? k0 + 128 : k0);   // the last turn re-reads its own keys: no branch around loads
-          st.step(s, vs, [&](int e) { return column<E4M3>(v, e); });
+          st.template step<false>(s, vs, [&](int e) { return column<E4M3>(v, e); });
         }
       }
     }
@@ -535,8 +565,11 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_k(KV8DecodeParams p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[a][r] = u0 + 16 * a + 4 * g + r < rows ? s[a][r] * sl2 : -INFINITY;
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)   // rows past the last one are it again, of weight 0: no infinity may meet that
+        if (u0 + 16 * (j >> 2) + 4 * g + (j & 3) >= rows) v[j] = vrow{};
       const float one[2] = {1.f, 1.f};
-      st.step(s, one, [&](int e) {
+      st.template step<true>(s, one, [&](int e) {
         bf16x8 o;
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = v[j][e];
@@ -636,20 +669,20 @@ __global__ __launch_bounds__(256) void kv8_combine_k(KV8DecodeParams p) {
     for (int e = 0; e < E; ++e) o[e] *= old;
     M = mx;
     const int n = min(64, shares - base);
-    for (int i0 = wave; i0 < n; i0 += 32) {   // eight loads in flight; past the end the last share again, with weight 0
+    for (int i0 = wave; i0 < n; i0 += 32) {   // eight loads in flight; past the end the last share again, not added
       float v[8][E], ai[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int i = min(i0 + 4 * u, n - 1);
         ai[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(a), i));
-        if (i0 + 4 * u >= n) ai[u] = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) v[u][e] = p.opart[slot(base + i) * D + (active ? lane * E + e : 0)];
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u)
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(ai[u], v[u][e], o[e]);
+        for (int e = 0; e < E; ++e)   // a sum of 0, not a weight of 0: that would make NaN of an infinity
+          o[e] = fmaf(ai[u], i0 + 4 * u < n ? v[u][e] : 0.f, o[e]);
     }
   }
   if (active) {

@@ -11,7 +11,7 @@ sequence b stored, ``KV8Cache`` holds
 with scale = max(amax / QMAX, 2^-126) and code = round(x * (1 / scale)) over the bf16 entries x of a block that has just
 been filled, QMAX = 127 (int8) or 448 (e4m3).  The open block stays bf16, so what n tokens leave in the cache does not
 depend on how they were grouped into appends.  A block with an entry that is not finite has the scale NaN and reads back
-as NaN.  Positions only grow (or restart at 0): an earlier token cannot be taken back out of a block that was quantised.
+as NaN; until it is full, its infinities are values like others.  Positions only grow (or restart at 0): an earlier token cannot be taken back out of a block that was quantised.
 
 GPU tensors run the HIP kernels (the extension must be present); CPU tensors run the PyTorch references below, which are
 also the oracles of tests/test_kv8_gpu.py.  There is no backward: operands that require grad are refused.

@@ -103,3 +103,23 @@ def logits64(logits, tokens, lengths, prompt, rep, pres, freq, bias, mask):
                 if not words[t // 32] >> (t % 32) & 1:
                     x[i, t] = -math.inf
     return x
+
+
+def infinities(cache, lengths):
+    """Infinities of either sign in the V of every sequence's open block, each in a column (head, d) of its own: in its
+    first and its last row, two of one sign in a column; and one of each sign in a column (their sum is NaN)."""
+    t = cache.v_tail.shape[1]
+    for b, n in enumerate(lengths):
+        if n % t:
+            last, v = n % t - 1, cache.v_tail[b]
+            v[0, 0, 3], v[last, 0, 4], v[0, 0, 5], v[last, 0, 5] = math.inf, -math.inf, -math.inf, -math.inf
+            if last:
+                v[0, 0, 9], v[last, 0, 9] = math.inf, -math.inf
+    return cache
+
+
+def assert_close64_inf(got, want, off):
+    """``assert_close64``, with infinities and NaN where (and of the sign that) the oracle has them."""
+    fin = torch.isfinite(want)
+    assert torch.equal(got.double()[~fin].nan_to_num(7.0), want[~fin].nan_to_num(7.0))
+    assert_close64(got[fin], want[fin], off[fin])
