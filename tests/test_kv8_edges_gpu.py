@@ -43,3 +43,56 @@ def test_decode_attention_infinities_in_the_open_block(dph_native, code, hq, hkv
     for b in (5, 6):   # alone: more shares of the row
         got = ops.kv8_decode_attention(qkv[b:b + 1], c.slot(b), pos[b:b + 1], hq, hkv)
         assert_close64_inf(got.cpu(), want[b:b + 1], off[b:b + 1])
+
+
+def test_graph_replays_over_rows_shared_by_workgroups(dph_native):
+    """Two captured append + attention steps whose rows several workgroups share (one of them with rows of fewer turns than
+    workgroups, one with more), each with its workspace in its graph's memory.  Replayed in turn with eager work between
+    them, across borders of turns (128 -> 129, 256 -> 257, 512 -> 513 keys) and of blocks, they equal eager steps bit for
+    bit: those divide the same lengths over as many workgroups."""
+    from kv8_oracle import tables
+
+    ops = _ops()
+    hq, d, t, cap = 8, 64, 16, 700
+    cos, sin = tables(d, cap, DEV)
+    hkv = [2, 4]
+    start = [_pos(120, 251, 500).to(DEV), (torch.arange(60) * 11 % 660).int().to(DEV)]
+    assert 60 * 4 * 6 > 512 > 3 * 2 * 6   # turns of 128 keys at the capacity against workgroups
+    caches = [_to(filled(ops.kv8_cache(len(p), cap, h, d, block=t), 40 + h), DEV) for p, h in zip(start, hkv)]
+    eager = [type(c)(*(x.clone(memory_format=torch.preserve_format) for x in c)) for c in caches]
+    pos, epos = [p.clone() for p in start], [p.clone() for p in start]
+
+    def step(x, c, p, h):
+        ops.kv8_append_(x, c, p, cos, sin, hq, h)
+        o = ops.kv8_decode_attention(x, c, p, hq, h)
+        p += 1
+        return o
+
+    bufs = [torch.zeros(len(p), 1, (hq + 2 * h) * d, dtype=torch.bfloat16, device=DEV) for p, h in zip(start, hkv)]
+    graphs, outs = [], []
+    for i in range(2):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(bufs[i].clone(), type(caches[i])(*(x.clone() for x in caches[i])), pos[i].clone(), hkv[i])
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(bufs[i], caches[i], pos[i], hkv[i]))
+        graphs.append(g)
+    for k in range(36):
+        x = [make_qkv(len(start[i]), 1, hq, hkv[i], d, 200 + 2 * k + i, DEV) for i in range(2)]
+        for i in (0, 1) if k % 2 else (1, 0):
+            bufs[i].copy_(x[i])
+            graphs[i].replay()
+        if k % 5 == 0:
+            torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], step(x[i], eager[i], epos[i], hkv[i])), (k, i)
+            assert torch.equal(bufs[i], x[i])
+        if k in (0, 17, 35):   # and are the attention of the cache as it stands
+            want, off = attention64(x[0].cpu(), _to(eager[0], "cpu"), epos[0].cpu() - 1, hq, hkv[0], d ** -0.5)
+            assert_close64_inf(outs[0].cpu(), want, off)
+    for i in range(2):
+        for name, a, b in zip(caches[i]._fields, caches[i], eager[i]):
+            assert torch.equal(a.float(), b.float()), name
