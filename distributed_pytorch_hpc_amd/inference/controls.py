@@ -75,6 +75,7 @@ class LogitProcessor:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.prompt = torch.zeros(batch, dtype=torch.int32, device=device)
         self.live = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._held = [0] * batch                                # lengths, known on the host
         self.penalties = torch.zeros(3, batch, device=device)   # repetition, presence, frequency
         self.penalties[0] = 1.0
         self.bias: Optional[torch.Tensor] = None                # [batch, V], with the first row that has one
@@ -88,7 +89,7 @@ class LogitProcessor:
         self.banned[i] = None if row is None else row == -math.inf
         self.controls[i] = controls
         self.tokens[i, :len(prompt)] = torch.as_tensor(list(prompt), dtype=torch.long)
-        self.lengths[i] = self.prompt[i] = len(prompt)
+        self.lengths[i] = self.prompt[i] = self._held[i] = len(prompt)
         self.live[i] = 1
         self.penalties[:, i] = torch.tensor([controls.repetition_penalty, controls.presence_penalty,
                                              controls.frequency_penalty])
@@ -101,7 +102,7 @@ class LogitProcessor:
         c, self.controls[i] = self.controls[i], None
         if c is None:
             return
-        self.lengths[i] = self.live[i] = 0
+        self.lengths[i] = self.live[i] = self._held[i] = 0
         if c.allowed is not None:
             self.mask[i] = -1
         if c.bias is not None:
@@ -113,12 +114,13 @@ class LogitProcessor:
         at = self.lengths.clamp(max=self.tokens.shape[1] - 1).long()[:, None]
         self.tokens.scatter_(1, at, torch.where(self.live > 0, tokens, 0)[:, None])
         self.lengths.add_(self.live).clamp_(max=self.tokens.shape[1])
+        self._held = [n if c is None else min(n + 1, self.tokens.shape[1]) for n, c in zip(self._held, self.controls)]
 
     def push_one(self, i: int, token: int) -> None:
         """Append one token to row i alone (the first token of a request that joins a running batch)."""
         n = min(int(self.lengths[i]), self.tokens.shape[1] - 1)
         self.tokens[i, n] = token
-        self.lengths[i] = n + 1
+        self.lengths[i] = self._held[i] = n + 1
 
     def restrict(self, i: int, generated: Sequence[int]) -> None:
         """Mask of row i's next token, given the ids generated so far; nothing to do for a row without ``allowed``."""
@@ -142,9 +144,10 @@ class LogitProcessor:
         mine = [c for c in self.controls[s] if c is not None]
         history = {}
         if any(c.penalizes for c in mine):
-            history = dict(tokens=self.tokens[s], lengths=self.lengths[s], prompt_lengths=self.prompt[s],
-                           repetition=self.penalties[0, s], presence=self.penalties[1, s],
-                           frequency=self.penalties[2, s])
+            # the columns in use, not the room: the kernel is chosen by the width of the history that it is given
+            history = dict(tokens=self.tokens[s, :max(self._held[s])], lengths=self.lengths[s],
+                           prompt_lengths=self.prompt[s], repetition=self.penalties[0, s],
+                           presence=self.penalties[1, s], frequency=self.penalties[2, s])
         bias = self.bias[s] if any(c.bias is not None for c in mine) else None
         mask = self.mask[s] if any(c.allowed is not None for c in mine) else None
         if not history and bias is None and mask is None:
