@@ -26,7 +26,7 @@ import torch
 from torch import nn
 
 from .. import ops
-from ..ops import decode as decode_ops
+from ..ops import _lib, decode as decode_ops, kv8 as kv8_ops
 from ..ops.rope import precompute_rope_tables
 from ..parallel import fused_layers
 
@@ -373,14 +373,14 @@ class Transformer(nn.Module):
 
 class KVCache:
     """Per-layer key / value cache of a Transformer for incremental decoding (serving; the reference model is
-    training-only).  ``k`` / ``v``: [n_layers, B, max_len, Hkv_local, head_dim]; ``pos``: int32 [B] device tensor =
-    tokens cached per sequence, read by the kernels (a captured decode graph advances it on the device alone).
+    training-only).  ``k`` / ``v``: [n_layers, B, max_len, Hkv_local, head_dim] (with ``kv_block`` a list of a layer's
+    [B, max_len, Hkv_local, head_dim] each); ``pos``: int32 [B] device tensor = tokens cached per sequence, read by the kernels (a captured decode graph advances it on the device alone).
     ``lengths`` mirrors pos on the host while it is known (None inside / after graph replays that the owner
     tracks itself).  ``slot(i)`` is a view of sequence i (prefill of prompts of different lengths).
     ``dtype=torch.float8_e4m3fn`` stores OCP e4m3 keys / values (value / ``kv_scale``): half the cache bytes.
     ``kv_block=T`` (16 / 32 / 64 / 128) stores int8 (``dtype=torch.int8``) or e4m3 codes with a scale for every block of T
     tokens of a KV head, taken from the block (ops.kv8): half the cache bytes without a scale to calibrate.  Its positions
-    only grow or restart at 0.
+    only grow or restart at 0, and on the GPU the head dim has to be 32, 64 or 128.
     Sized for HBM: 7B at 4 096 tokens is 2 GiB per sequence in bf16."""
 
     def __init__(self, model: "Transformer", batch: int, max_len: int, device=None, dtype: torch.dtype | None = None,
@@ -398,6 +398,9 @@ class KVCache:
         if kv_block is not None:
             if kv_scale != 1.0:
                 raise ValueError("KVCache: kv_block takes its scales from the blocks, kv_scale must stay 1")
+            if device.type == "cuda" and not _lib.reference_mode() and args.head_dim not in kv8_ops.HEAD_DIMS:
+                raise ValueError(f"KVCache: kv_block on the GPU needs a head dim of {kv8_ops.HEAD_DIMS}, the model has "
+                                 f"{args.head_dim}")
             self.blocks = [ops.kv8_cache(batch, max_len, hkv, args.head_dim, dtype, kv_block, device)
                            for _ in range(n_layers)]
             self.k, self.v = [c.k for c in self.blocks], [c.v for c in self.blocks]

@@ -11,7 +11,8 @@ sequence b stored, ``KV8Cache`` holds
 with scale = max(amax / QMAX, 2^-126) and code = round(x * (1 / scale)) over the bf16 entries x of a block that has just
 been filled, QMAX = 127 (int8) or 448 (e4m3).  The open block stays bf16, so what n tokens leave in the cache does not
 depend on how they were grouped into appends.  A block with an entry that is not finite has the scale NaN and reads back
-as NaN; until it is full, its infinities are values like others.  Positions only grow (or restart at 0): an earlier token cannot be taken back out of a block that was quantised.
+as NaN; until it is full, its infinities are values like others.  Positions only grow (or restart at 0): an earlier token
+cannot be taken back out of a block that was quantised.
 
 GPU tensors run the HIP kernels (the extension must be present); CPU tensors run the PyTorch references below, which are
 also the oracles of tests/test_kv8_gpu.py.  There is no backward: operands that require grad are refused.
@@ -27,6 +28,7 @@ from . import _lib
 from .decode import FP8_KV, FP8_MAX, _split
 
 TINY_SCALE = 2.0 ** -126
+HEAD_DIMS = (32, 64, 128)   # of the HIP kernels; the references take any even one
 QMAX = {torch.int8: 127.0, FP8_KV: FP8_MAX}
 
 
@@ -70,7 +72,8 @@ def _no_grad(name: str, *ts) -> None:
 
 
 def _check(cache: KV8Cache, pos, qkv=None, n_heads: int = 0, n_kv_heads: int = 0, tables=()) -> None:
-    """The refusals of the native operators for the CPU path."""
+    """The refusals of the native operators for the CPU path, but for what only kernels need: HEAD_DIMS, strides, alignment
+    and operands that lie apart."""
     k, v, ks, vs, kt, vt = cache
     b, smax, h, d = k.shape
     t = kt.shape[1]

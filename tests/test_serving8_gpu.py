@@ -97,3 +97,16 @@ def test_processor_keeps_history_on_the_device(dph_native):
         outs.append((p.tokens.cpu(), p.lengths.cpu(), p(z).cpu(), p(z[1:2], row=1).cpu()))
     for a, b in zip(*outs):
         torch.testing.assert_close(a, b, rtol=0, atol=8 * 2.0 ** -24 * 4)   # eight roundings of values below 4
+
+
+def test_unsupported_head_dim_is_refused_with_the_cache(dph_native):
+    """Not at the first append: a model with heads of 16 gets no block-scaled cache on the GPU, and keeps its bf16 one."""
+    from distributed_pytorch_hpc_amd.inference import Generator
+    from distributed_pytorch_hpc_amd.models.llama2 import KVCache, ModelArgs, build_llama
+
+    m = build_llama(ModelArgs(dim=64, n_layers=1, n_heads=4, n_kv_heads=2, vocab_size=96, multiple_of=32, max_seq_len=64),
+                    device="cuda", dtype=torch.bfloat16)
+    for make in (KVCache, Generator):
+        with pytest.raises(ValueError, match="head dim"):
+            make(m, 2, 32, dtype=torch.int8, kv_block=16)
+    KVCache(m, 2, 32)
