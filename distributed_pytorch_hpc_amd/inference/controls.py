@@ -16,12 +16,20 @@ import torch
 
 from .. import ops
 
+# What is sampled from has to stay finite where a token is allowed (softmax makes NaN of a row without a finite entry, and
+# sampling from that ends a process on the GPU).  Logits below 2^36 times a repetition penalty of 2^64, less 2^31 copies
+# of a token times 2^64, plus a bias of 2^100 stay below 2^102 in 32 and in 16 bits, and below 2^127 when divided by a
+# temperature of 2^-25.
+MAX_PENALTY = 2.0 ** 64
+MAX_BIAS = 2.0 ** 100
+
 
 @dataclass
 class LogitControls:
     """repetition_penalty r > 0: the logit of every token of the prompt or output is divided by r if positive, else
-    multiplied; frequency / presence: subtracted for each generated copy / once; bias: {token: value} or fp32 [V], added;
-    allowed: called with the generated ids before each token, returns a bool [V] tensor (True: may be sampled) or None for
+    multiplied; frequency / presence: subtracted for each generated copy / once (penalties of up to 2^64, repetition also
+    of at least 2^-64); bias: {token: value} or fp32 [V], added (below -2^100, as a type's lowest value is, it stands for
+    -inf: never this token); allowed: called with the generated ids before each token, returns a bool [V] tensor (True: may be sampled) or None for
     no limit."""
     repetition_penalty: float = 1.0
     presence_penalty: float = 0.0
@@ -30,10 +38,10 @@ class LogitControls:
     allowed: Optional[Callable[[Sequence[int]], Optional[torch.Tensor]]] = None
 
     def __post_init__(self):
-        if not 0.0 < self.repetition_penalty < math.inf:
-            raise ValueError(f"LogitControls: repetition_penalty must be positive, got {self.repetition_penalty}")
-        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
-            raise ValueError("LogitControls: penalties must be finite")
+        if not 1 / MAX_PENALTY <= self.repetition_penalty <= MAX_PENALTY:
+            raise ValueError(f"LogitControls: repetition_penalty must be in [2^-64, 2^64], got {self.repetition_penalty}")
+        if not (abs(self.presence_penalty) <= MAX_PENALTY and abs(self.frequency_penalty) <= MAX_PENALTY):
+            raise ValueError("LogitControls: penalties must be finite, 2^64 at most")
 
     @property
     def penalizes(self) -> bool:
@@ -43,17 +51,18 @@ class LogitControls:
         if self.bias is None:
             return None
         if isinstance(self.bias, torch.Tensor):
-            row = self.bias.detach().float().cpu()
+            row = self.bias.detach().cpu()
             if tuple(row.shape) != (vocab,):
                 raise ValueError(f"LogitControls: bias must have {vocab} entries, got {tuple(row.shape)}")
         else:
-            row = torch.zeros(vocab)
+            row = torch.zeros(vocab, dtype=torch.float64)
             for t, v in self.bias.items():
                 if not 0 <= t < vocab:
                     raise ValueError(f"LogitControls: bias for token {t} outside the vocabulary of {vocab}")
                 row[t] = v
-        if bool(row.isnan().any() | (row == math.inf).any()):
-            raise ValueError("LogitControls: biases must be finite or -inf")
+        if bool((row.isnan() | (row > MAX_BIAS)).any()):
+            raise ValueError("LogitControls: biases must be 2^100 at most, or -inf")
+        row = row.masked_fill(row < -MAX_BIAS, -math.inf).float()
         if bool((row == -math.inf).all()):
             raise ValueError("LogitControls: biases of -inf leave no token")
         return row

@@ -44,3 +44,55 @@ def test_processor_hands_over_the_history_in_use(monkeypatch):
     proc.stop(0)
     proc(z)
     assert widths == [2, 4, 5, 6, 3, 9, 9, 0]
+
+
+LOWEST = [torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min, -1e39, -1e300]
+
+
+@pytest.mark.parametrize("low", LOWEST)
+@pytest.mark.parametrize("temperature", [0.0, 0.5])
+def test_a_bias_of_the_lowest_value_bans_a_token(low, temperature):
+    """As -inf does: the others are sampled, and where none is left the call is refused before it has sampled."""
+    from distributed_pytorch_hpc_amd.inference import ContinuousBatcher, Generator, LogitControls
+
+    m = _model()
+    g = Generator(m, 1, 16)
+    for bias in ({t: low for t in range(50)}, low * (torch.arange(97) < 50).double()):
+        out = g.generate([[1]], 8, temperature=temperature, controls=LogitControls(bias=bias, presence_penalty=1.0),
+                         generator=torch.Generator().manual_seed(0))
+        assert min(out[0][1:]) >= 50
+        with pytest.raises(ValueError, match="no token"):
+            g.generate([[1]], 2, temperature=temperature,
+                       controls=LogitControls(bias=bias, allowed=lambda made: torch.arange(97) < 50))
+    for c in (g.generate, ContinuousBatcher(g).submit):
+        with pytest.raises(ValueError, match="no token"):
+            c([[1]] if c == g.generate else [1], 2, controls=LogitControls(bias=torch.full((97,), low, dtype=torch.float64)))
+
+
+@pytest.mark.parametrize("kw", [dict(repetition_penalty=1e-50), dict(repetition_penalty=1e39), dict(repetition_penalty=1e-30),
+                                dict(presence_penalty=1e39), dict(frequency_penalty=-1e39), dict(presence_penalty=-1e300),
+                                dict(frequency_penalty=3e38)])
+def test_penalties_that_leave_32_bits_are_refused(kw):
+    """1e-50 is zero in 32 bits, 1e39 infinite, and a few copies of a token times 3e38 are."""
+    from distributed_pytorch_hpc_amd.inference import LogitControls
+
+    with pytest.raises(ValueError, match="LogitControls"):
+        LogitControls(**kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_controls_leave_finite_logits(dtype):
+    from distributed_pytorch_hpc_amd.inference import LogitControls, LogitProcessor
+
+    z = torch.linspace(-2.0 ** 35, 2.0 ** 35, 20)[None].to(dtype)
+    for sign in (1, -1):
+        for rep in (2.0 ** 64, 2.0 ** -64):
+            p = LogitProcessor(1, 40, 20, "cpu")
+            p.start(0, list(range(20)), LogitControls(rep, sign * 2.0 ** 64, sign * 2.0 ** 64,
+                                                      torch.full((20,), -sign * 2.0 ** 100)))
+            for t in range(20):
+                p.push(torch.tensor([t]))
+            y = p(z)
+            assert torch.isfinite(y).all() and torch.isfinite(y.float() / 2.0 ** -25).all()
+    with pytest.raises(ValueError, match="biases"):
+        LogitProcessor(1, 4, 20, "cpu").start(0, [1], LogitControls(bias={3: 2.0 ** 101}))
