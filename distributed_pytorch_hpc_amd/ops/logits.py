@@ -3,7 +3,7 @@
 Per row of logits x [N, V], with the history tokens[n, :lengths[n]] whose first prompt_lengths[n] ids are the prompt's,
 in this order and in 32 bits:
 
-  token in the history   x = x / repetition if x > 0 else x * repetition
+  token in the history   x = x / repetition if x > 0 else x * repetition   (the kernel: x * (1 / repetition))
   c > 0 generated copies x = x - (frequency * c + presence)
   bias                   x = x + bias
   mask bit 0             x = -inf

@@ -176,3 +176,26 @@ def test_more_rows_than_wide_workgroups(dph_native):
                              presence=(torch.arange(n, device=DEV) % 5).float())
     want = x.scatter_add(1, tokens, -(torch.arange(n, device=DEV) % 5).float()[:, None])
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("v", [64, 65])
+def test_repetition_penalties_whose_reciprocal_leaves_32_bits(dph_native, v):
+    """1 / r is infinite for r = 2^-140 and has lost digits for r = 1.3 * 2^127, x / r is neither: one rounding from it.
+    A penalty of infinity leaves zero, one of zero infinity."""
+    r = torch.tensor([2.0 ** -140, 1.3 * 2.0 ** 127, 2.0 ** -126, 2.0 ** 126, math.inf, 0.0])
+    x = torch.linspace(1, 1000, v).repeat(6, 1)
+    x[0] *= 2.0 ** -30
+    x[2] *= 2.0 ** -30
+    x[1] *= 2.0 ** 100
+    x[3] *= 2.0 ** 100
+    x[:4, ::3] *= -2.0 ** -20   # times r, not divided
+    tokens = torch.arange(v).repeat(6, 1)
+    got = _run(x, tokens, torch.full((6,), v, dtype=torch.int32), dict(repetition=r)).cpu()
+    want = torch.where(x > 0, x.double() / r[:, None].double(), x.double() * r[:, None].double())
+    assert (got[4] == 0).all() and (got[5] == math.inf).all()
+    # half a step of the result (2^-24, and of the least subnormal), for the reciprocal a second rounding
+    err = (got[:4].double() - want[:4]).abs()
+    fits = want[:4].float().isfinite()
+    assert (err <= 2 * 2.0 ** -24 * want[:4].abs() * (1 + 2.0 ** -20) + 2.0 ** -149)[fits].all()
+    assert (got[:4].isinf() & (got[:4].sign() == want[:4].sign()))[~fits].all()
+    assert fits[0].all() and fits[2].all()
