@@ -96,3 +96,24 @@ def test_graph_replays_over_rows_shared_by_workgroups(dph_native):
     for i in range(2):
         for name, a, b in zip(caches[i]._fields, caches[i], eager[i]):
             assert torch.equal(a.float(), b.float()), name
+
+
+@pytest.mark.parametrize("cap,t", [(1, 16), (10, 64), (127, 128)])
+def test_capacity_below_one_block(dph_native, cap, t):
+    """No block ever fills and there is no scale: everything lives in the open block."""
+    from kv8_oracle import tables
+
+    ops = _ops()
+    cos, sin = tables(64, cap, "cpu")
+    ref = ops.kv8_cache(2, cap, 2, 64, block=t)
+    got = _to(ref, DEV)
+    assert ref.k_scale.shape == (2, 0, 2)
+    x = make_qkv(2, cap, 6, 2, 64, 3, "cpu")
+    gx, pos = x.to(DEV), _pos(0, 0)
+    ops.kv8_append_(x, ref, pos, cos, sin, 6, 2)
+    ops.kv8_append_(gx, got, pos.to(DEV), cos.to(DEV), sin.to(DEV), 6, 2)
+    assert torch.equal(gx.cpu(), x) and torch.equal(got.v_tail.cpu(), ref.v_tail) and torch.equal(got.k_tail.cpu(), ref.k_tail)
+    pos += cap - 1
+    want, off = attention64(x[:, -1:], ref, pos, 6, 2, 0.125)
+    assert_close64_inf(ops.kv8_decode_attention(gx[:, -1:], got, pos.to(DEV), 6, 2).cpu(), want, off)
+    assert torch.equal(ops.kv8_read(got, pos.to(DEV) + 1, cap)[0].cpu(), ops.kv8_read(ref, pos + 1, cap)[0])
