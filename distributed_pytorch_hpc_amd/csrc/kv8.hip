@@ -218,9 +218,9 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
 // 8-bit -> bf16 conversion is the largest part of the arithmetic: about 1.5 instructions an element, a third of what the
 // vector units can do in the time that the bytes take.  Four waves of a workgroup share a turn of 128 keys and merge over
 // LDS; where several workgroups share a row, they leave unnormalised sums for kv8_combine_k.
-// Measured: 16 sequences of 1000 to 4000 tokens, 32 / 32 heads, 328 MB: 61 us, 5.35 TB/s (a streaming read of that size:
-// 5.8 to 6.0); 32 of 4000 to 8100 tokens, 64 / 8 heads, 398 MB: 74 us; one of 32 002 tokens, 64 / 8 heads: 15.8 us; one of
-// 2346 tokens, 32 / 32 heads: 8.2 us.  The merge adds 3.6 to 5.6 us and a launch.  One thread per 8 elements and key instead
+// Measured (kernel trace): 16 sequences of 1000 to 4000 tokens, 32 / 32 heads, 328 MB: 63 us, 5.2 TB/s (a streaming read of
+// that size: 5.8 to 6.0); 32 of 4000 to 8100 tokens, 64 / 8 heads, 398 MB: 75.5 us; one of 32 002 tokens, 64 / 8 heads:
+// 15.8 us; one of 2346 tokens, 32 / 32 heads: 8.6 us.  The merge adds 3.5 to 5.7 us and a launch.  One thread per 8 elements and key instead
 // of matrix tiles: 399, 964, 2095 and 152 us.
 template <int D>
 struct Raw {   // a lane's share of the codes of one key (K) and of one key's part of a head (V)
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(256, 2) void kv8_decode_k(KV8DecodeParams p) {
 }
 
 // One workgroup per (sequence, query head) joins the shares of a row that several workgroups had: its waves take them in
-// turns, then merge.  D / 64 (at least 1) elements a lane.  3.6 (32 rows) to 5.6 us (2048 rows): latency.
+// turns, then merge.  D / 64 (at least 1) elements a lane.  3.5 (32 rows) to 5.7 us (2048 rows): latency.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_combine_k(KV8DecodeParams p) {
   constexpr int E = D >= 64 ? D / 64 : 1;
@@ -778,7 +778,8 @@ void kv8_append(const KV8AppendParams& p, hipStream_t st) {
 #undef DPH_KV8_APP
 }
 
-// Workgroups of a call: three to a CU (what the registers allow at once), or one for each turn that the longest sequences could have.
+// Workgroups of a call: two to a CU (what the registers allow at once; memory is busy with them), or one for each turn that
+// the longest sequences could have.
 int kv8_decode_workgroups(int64_t turns) { return (int)std::min<int64_t>(turns, 512); }
 
 void kv8_decode_attention(const KV8DecodeParams& p, hipStream_t st) {

@@ -3,9 +3,12 @@
 //   masked: x = -inf.
 // A workgroup owns a segment of one row's vocabulary and counts that segment's tokens of the history in LDS -- integer
 // atomics, so the order of arrival does not matter -- between asking for its logits and using them.  No state is kept from
-// call to call: reading the ids again costs 8 bytes a token of the history, a [N, V] table of counts 4 bytes a logit.
-// Bound by latency (launch, ids, LDS) and then by memory: one row of 32 000 with 300 ids 3.4 us; 64 rows, bf16, 4000 ids
-// each, bias and mask 7.1 us, 2.6 TB/s of its 19 MB; 64 rows of fp32 with a mask alone 6.2 us.  Loads under conditions of
+// call to call, so no [N, V] table of counts has to follow a request through its slot.  The price: every segment of a row
+// reads the row's ids again, 8 bytes each, 4 (1024 threads) or 16 times (256) at V = 32 000, mostly from L2; at 4000 ids
+// that is the 128 kB that a row of such a table has, or four times as much.
+// Bound by latency (launch, lengths, ids, LDS and two barriers, one after the other) and then by memory: one row of 32 000
+// with 300 ids 3.6 us; 64 rows, bf16, 4000 ids each, bias and mask 7.2 us, 2.6 TB/s of its 19 MB, of which the history is
+// about 1 us: 64 rows of fp32 with a mask alone take 6.2 us (replays of captured calls).  Loads under conditions of
 // their own, each waiting for the last, took 23 us.
 #include "dph_common.h"
 #include "kernels.h"
