@@ -118,9 +118,10 @@ def kv8_append_reference(qkv, cache: KV8Cache, pos, cos, sin, n_heads: int, n_kv
     t, smax = cache.block, cache.k.shape[1]
     q, k, v = _split(qkv, n_heads, n_kv_heads, cache.k.shape[-1])
     s = qkv.shape[1]
-    for b, p in enumerate(pos.tolist()):
+    for b, p in enumerate(pos.tolist()):   # before anything is stored
         if p < 0 or p + s > smax:
             raise ValueError(f"kv8 cache overflow: sequence {b} at {p} + {s} > capacity {smax}")
+    for b, p in enumerate(pos.tolist()):
         for x in (q, k):
             x[b].copy_(_rotate64(x[b], cos[p:p + s], sin[p:p + s]))
         first, end = p // t, (p + s) // t

@@ -22,3 +22,17 @@ def test_decode_reference_with_infinities_in_the_open_block(code):
     want, off = attention64(qkv, cache, pos, 8, 2, 0.125)
     assert torch.isinf(want).any() and want.isnan().any()
     assert_close64_inf(ops.kv8_decode_attention(qkv, cache, pos, 8, 2), want, off)
+
+
+def test_a_refused_append_leaves_everything_as_it_was():
+    """The second sequence has no room: the first one's open block is not quantised away under its unchanged position."""
+    from kv8_oracle import tables
+
+    ops = _ops()
+    cos, sin = tables(32, 40, "cpu")
+    cache, x = filled(ops.kv8_cache(2, 40, 2, 32, block=16), 1), make_qkv(2, 3, 4, 2, 32, 0, "cpu")
+    before = [t.clone() for t in (*cache, x)]
+    for pos in ([14, 38], [14, -1]):
+        with pytest.raises(ValueError, match="overflow"):
+            ops.kv8_append_(x, cache, torch.tensor(pos, dtype=torch.int32), cos, sin, 4, 2)
+        assert all(torch.equal(a.float(), b.float()) for a, b in zip((*cache, x), before))
