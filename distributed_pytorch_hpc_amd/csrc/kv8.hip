@@ -220,8 +220,8 @@ __global__ __launch_bounds__(256) void kv8_append_k(KV8AppendParams p, int nblk,
 // LDS; where several workgroups share a row, they leave unnormalised sums for kv8_combine_k.
 // Measured (kernel trace): 16 sequences of 1000 to 4000 tokens, 32 / 32 heads, 328 MB: 63 us, 5.2 TB/s (a streaming read of
 // that size: 5.8 to 6.0); 32 of 4000 to 8100 tokens, 64 / 8 heads, 398 MB: 75.5 us; one of 32 002 tokens, 64 / 8 heads:
-// 15.8 us; one of 2346 tokens, 32 / 32 heads: 8.6 us.  The merge adds 3.5 to 5.7 us and a launch.  One thread per 8 elements and key instead
-// of matrix tiles: 399, 964, 2095 and 152 us.
+// 15.8 us; one of 2346 tokens, 32 / 32 heads: 8.6 us.  The merge adds 3.5 to 5.7 us and a launch.  One thread per 8
+// elements and key instead of matrix tiles: 399, 964, 2095 and 152 us.
 template <int D>
 struct Raw {   // a lane's share of the codes of one key (K) and of one key's part of a head (V)
   typedef typename std::conditional<D >= 64, u32x4, uint2>::type K;
@@ -267,7 +267,7 @@ __device__ __forceinline__ bf16x8 column(const V (&v)[8], int e) {
   return o;
 }
 
-// 2^x, zero below 2^-126: a weight that small adds nothing
+// 2^x, zero below 2^-126: a weight that small adds nothing (and makes NaN of an infinity, as any weight of zero does)
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ bf16x8 finite_or_zero(bf16x8 v) {
